@@ -1,0 +1,499 @@
+// The AdamW step over many tensors at once, with moments in 32 or in 8 bits, and the norm of many gradients.
+//
+//   g' = g min(1, max_norm / (norm + 1e-6))            (where clipping is asked for)
+//   m' = b1 m + (1 - b1) g',  v' = b2 v + (1 - b2) g'^2
+//   p' = p (1 - lr wd) - lr / (1 - b1^t) * m' / (sqrt(v') / sqrt(1 - b2^t) + eps)
+//
+// in fp32, each product and sum rounded by itself.  Bound: HBM, 28 bytes an element for fp32 parameters with
+// 32-bit moments, 16 with 8-bit ones, 10 for bf16 parameters and gradients with 8-bit moments.
+//
+// 8-bit moments.  256 elements (a wave's 64 lanes with 4 each: its maximum needs no LDS) share two powers of
+// two.  m is a sign, 4 exponent and 3 mantissa bits under 2^em, v 5 and 3 bits without a sign under 2^ev:
+//   |m| = 2^em * {n 2^-9 (e = 0), (8 + n) 2^(e - 10)},  v = 2^ev * {n 2^-33 (e = 0), (8 + n) 2^(e - 34)}
+// (v's range, 2^-33 to 1.75, is about the square of m's, so that sqrt(v) keeps up with m).  Both layouts are
+// fp32's with the lower mantissa bits cut off, once the number is scaled so that the code's exponent field is
+// fp32's: bits >> 20 is the code, subnormals included, and bits << 20 the number.  A block whose largest value
+// has a mantissa of 1.75 or more takes the next exponent, so no finite value reaches the codes of NaN (m) and
+// infinity (v); these keep what overflowed visible.
+//
+// The cut is random: 20 hashed bits (12 for m) are added below the code's last bit.  A step changes v by
+// (1 - b2) of itself, 0.1 % at b2 = 0.999, against half a code's 6 %: rounding to nearest would leave v where it
+// is for good, rounding at random keeps its mean.  The same holds for bf16 parameters (half a step is 2^-9 of
+// the value, lr is 1e-4).  A v that is not zero does not become zero: m / sqrt(v) would jump.
+// The 32 bits belong to (seed, step, the tensor's place, the element's place), so a run can be repeated.
+#include <type_traits>
+
+#include "common.h"
+
+namespace iadmm {
+
+constexpr int kPer = 48;          // tensors of a launch: they travel in its arguments (3.5 KB of 4)
+constexpr int kBlock8 = 256;      // elements under one pair of exponents
+constexpr int kNormPer = 128, kNormBlocks = 1024;
+
+enum { kHalfP = 1, kHalfG = 2 };  // AdamTensor::flags
+
+struct AdamTensor {
+  void* p;
+  const void* g;
+  void *m, *v, *e;
+  int64_t n;
+  float step_size, ibc2;
+  uint32_t key;
+  uint32_t first;  // its first workgroup
+  int flags, slot;
+};
+
+struct AdamLaunch {
+  AdamTensor t[kPer];
+  const float* norm;     // or null
+  const float4* table;   // step size, 1 / sqrt(1 - b2^t), 1 - lr wd, key of each tensor, or null: those of t
+  float decay, b1, ob1, b2, ob2, eps, max_norm;
+  int count;
+};
+
+// 32 well-mixed bits of 32: two odd multipliers between shifts, chosen by search for the least bias of any
+// output bit's flip under any input bit's (0.4 % at most over 200 000 inputs).
+__host__ __device__ inline uint32_t mix32(uint32_t x) {
+  x ^= x >> 16;
+  x *= 0xDEFBD895u;
+  x ^= x >> 15;
+  x *= 0x066B4493u;
+  return x ^ (x >> 16);
+}
+__host__ __device__ inline uint32_t step_key(uint64_t seed, uint64_t step, int slot) {
+  uint32_t k = mix32(static_cast<uint32_t>(seed) + 0x9E3779B9u);
+  k = mix32(k ^ static_cast<uint32_t>(seed >> 32));
+  k = mix32(k + static_cast<uint32_t>(step));
+  return mix32(k ^ static_cast<uint32_t>(slot));
+}
+
+// Four neighbouring elements, at any address that the type may have; what lies behind the end is 0.
+template <typename T> struct Quad { T v[4]; };
+template <typename T> IADMM_DEV Quad<T> load_quad(const T* p, int64_t left) {
+  Quad<T> r;
+  if (left >= 4) {
+    __builtin_memcpy(&r, p, sizeof(r));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r.v[j] = j < left ? p[j] : static_cast<T>(0);
+  }
+  return r;
+}
+template <typename T> IADMM_DEV void store_quad(T* p, const Quad<T>& r, int64_t left) {
+  if (left >= 4) {
+    __builtin_memcpy(p, &r, sizeof(r));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < left) p[j] = r.v[j];
+  }
+}
+
+IADMM_DEV float bits_f(uint32_t b) { return __uint_as_float(b); }
+IADMM_DEV bool is_finite(float x) { return fabsf(x) < __builtin_inff(); }
+
+IADMM_DEV float decode_m(uint32_t c, int e) {
+  const float a = __builtin_amdgcn_ldexpf(bits_f((c & 127u) << 20), e + 120);
+  return bits_f(__float_as_uint((c & 127u) == 127u ? __builtin_nanf("") : a) | (c & 128u) << 24);
+}
+IADMM_DEV float decode_v(uint32_t c, int e) {
+  return c == 255u ? __builtin_inff() : __builtin_amdgcn_ldexpf(bits_f(c << 20), e + 96);
+}
+IADMM_DEV uint32_t encode_m(float m, int e, uint32_t bits) {
+  const uint32_t a = __float_as_uint(__builtin_amdgcn_ldexpf(fabsf(m), -e - 120));
+  uint32_t c = (a + (bits >> 20 << 8)) >> 20;
+  c = c < 126u ? c : 126u;
+  return (is_finite(m) ? c : 127u) | (m < 0.0f ? 128u : 0u);
+}
+IADMM_DEV uint32_t encode_v(float v, int e, uint32_t bits) {
+  const uint32_t a = __float_as_uint(__builtin_amdgcn_ldexpf(v, -e - 96));
+  uint32_t c = (a + (bits & 0xFFFFFu)) >> 20;
+  c = c < 254u ? c : 254u;
+  c = c == 0u && v > 0.0f ? 1u : c;
+  return is_finite(v) ? c : 255u;
+}
+IADMM_DEV int block_exponent(uint32_t top, int shift, int low, int high) {
+  const int e = static_cast<int>((top + 0x200000u) >> 23) - 127 - shift;
+  return e < low ? low : (e > high ? high : e);
+}
+IADMM_DEV uint32_t wave_umax(uint32_t v) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) {
+    const uint32_t w = static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), o, kWave));
+    v = w > v ? w : v;
+  }
+  return v;
+}
+
+// Which of the launch's tensors this workgroup serves: the last whose first workgroup is not behind it.
+template <typename L> IADMM_DEV int find_tensor(const L& a, uint32_t block) {
+  int at = 0;
+  for (int k = threadIdx.x % kWave; k < a.count; k += kWave)
+    if (a.t[k].first <= block) at = k;
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) {
+    const int w = __shfl_xor(at, o, kWave);
+    at = w > at ? w : at;
+  }
+  return __builtin_amdgcn_readfirstlane(at);
+}
+
+struct AdamScalars {
+  float step_size, ibc2, decay, clip;
+  uint32_t key;
+  bool clipped;
+};
+
+// QUADS x 256 elements per wave, a workgroup's four waves beside each other.
+template <typename P, typename G, bool EIGHT, int QUADS>
+IADMM_DEV void adam_chunk(const AdamLaunch& a, const AdamTensor& t, const AdamScalars& s) {
+  using S = typename std::conditional<EIGHT, uint8_t, float>::type;
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int64_t at = (static_cast<int64_t>(blockIdx.x - t.first) * 4 + wave) * (QUADS * 256);
+  P* p = static_cast<P*>(t.p);
+  const G* g = static_cast<const G*>(t.g);
+  S *m = static_cast<S*>(t.m), *v = static_cast<S*>(t.v);
+  int8_t* e = static_cast<int8_t*>(t.e);
+  Quad<P> qp[QUADS];
+  Quad<G> qg[QUADS];
+  Quad<S> qm[QUADS], qv[QUADS];
+  int em[QUADS], ev[QUADS];
+#pragma unroll
+  for (int u = 0; u < QUADS; ++u) {
+    const int64_t i = at + u * 256 + lane * 4, left = t.n - i;
+    qp[u] = load_quad(p + i, left);
+    qg[u] = load_quad(g + i, left);
+    qm[u] = load_quad(m + i, left);
+    qv[u] = load_quad(v + i, left);
+    em[u] = ev[u] = 0;
+    if (EIGHT && at + u * 256 < t.n) {
+      em[u] = e[(at + u * 256) / kBlock8 * 2];
+      ev[u] = e[(at + u * 256) / kBlock8 * 2 + 1];
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < QUADS; ++u) {
+    if (at + u * 256 >= t.n) break;  // (the whole wave)
+    const int64_t i = at + u * 256 + lane * 4, left = t.n - i;
+    float fm[4], fv[4];
+    uint32_t bits[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float gr = static_cast<float>(qg[u].v[j]);
+      if (s.clipped) gr = gr * s.clip;
+      float om, ov;
+      if constexpr (EIGHT) {
+        om = decode_m(qm[u].v[j], em[u]);
+        ov = decode_v(qv[u].v[j], ev[u]);
+      } else {
+        om = qm[u].v[j];
+        ov = qv[u].v[j];
+      }
+      fm[j] = a.b1 * om + a.ob1 * gr;
+      fv[j] = a.b2 * ov + a.ob2 * (gr * gr);
+      const float d = sqrtf(fv[j]) * s.ibc2 + a.eps;
+      const float np = static_cast<float>(qp[u].v[j]) * s.decay - s.step_size * (fm[j] / d);
+      if constexpr (EIGHT || sizeof(P) == 2) {
+        const int64_t k = i + j;
+        bits[j] = mix32((static_cast<uint32_t>(k) + static_cast<uint32_t>(k >> 32) * 0x9E3779B9u) ^ s.key);
+      }
+      if constexpr (sizeof(P) == 2) {
+        const uint32_t b = (__float_as_uint(np) + (bits[j] >> 16)) >> 16;
+        const uint16_t h = static_cast<uint16_t>(np != np ? 0x7FC0u : b);
+        __builtin_memcpy(&qp[u].v[j], &h, 2);
+      } else {
+        qp[u].v[j] = np;
+      }
+    }
+    store_quad(p + i, qp[u], left);
+    if constexpr (EIGHT) {
+      uint32_t tm = 0, tv = 0;  // (elements behind the end are 0)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t bm = is_finite(fm[j]) ? __float_as_uint(fabsf(fm[j])) : 0u;
+        const uint32_t bv = is_finite(fv[j]) ? __float_as_uint(fv[j]) : 0u;
+        tm = bm > tm ? bm : tm;
+        tv = bv > tv ? bv : tv;
+      }
+      const int ne = block_exponent(wave_umax(tm), 8, -117, 120), nv = block_exponent(wave_umax(tv), 0, -93, 127);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        qm[u].v[j] = static_cast<uint8_t>(encode_m(fm[j], ne, bits[j]));
+        qv[u].v[j] = static_cast<uint8_t>(encode_v(fv[j], nv, bits[j]));
+      }
+      if (lane == 0) {
+        e[(at + u * 256) / kBlock8 * 2] = static_cast<int8_t>(ne);
+        e[(at + u * 256) / kBlock8 * 2 + 1] = static_cast<int8_t>(nv);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) qm[u].v[j] = fm[j], qv[u].v[j] = fv[j];
+    }
+    store_quad(m + i, qm[u], left);
+    store_quad(v + i, qv[u], left);
+  }
+}
+
+template <bool EIGHT, int QUADS> __global__ void __launch_bounds__(256) adam_kernel(const AdamLaunch a) {
+  const int k = find_tensor(a, blockIdx.x);
+  const AdamTensor& t = a.t[k];
+  AdamScalars s{t.step_size, t.ibc2, a.decay, 1.0f, t.key, a.norm != nullptr};
+  if (a.table) {
+    const float4 f = a.table[k];
+    s.step_size = f.x;
+    s.ibc2 = f.y;
+    s.decay = f.z;
+    s.key = __float_as_uint(f.w);
+  }
+  if (a.norm) {
+    const float c = a.max_norm / (*a.norm + 1e-6f);
+    s.clip = c > 1.0f ? 1.0f : c;  // (a norm that is NaN reaches every parameter)
+  }
+  switch (t.flags) {
+    case 0: adam_chunk<float, float, EIGHT, QUADS>(a, t, s); break;
+    case kHalfG: adam_chunk<float, __bf16, EIGHT, QUADS>(a, t, s); break;
+    case kHalfP: adam_chunk<__bf16, float, EIGHT, QUADS>(a, t, s); break;
+    default: adam_chunk<__bf16, __bf16, EIGHT, QUADS>(a, t, s); break;
+  }
+}
+
+// Steps that live on the device (a captured step has to count by itself): counts, and writes what the
+// parameters' kernel needs of the count.
+struct AdamCount {
+  int slot[kPer];
+  int64_t* steps;
+  const float* lr;
+  double lr_host, b1, b2, decay;
+  uint64_t seed;
+  float4* table;
+  int count;
+};
+__global__ void adam_count_kernel(const AdamCount a) {
+  const int k = threadIdx.x;
+  if (k >= a.count) return;
+  const int64_t step = a.steps[a.slot[k]] + 1;
+  a.steps[a.slot[k]] = step;
+  const double lr = a.lr ? static_cast<double>(*a.lr) : a.lr_host, t = static_cast<double>(step);
+  a.table[k] = make_float4(static_cast<float>(lr / (1.0 - pow(a.b1, t))), static_cast<float>(1.0 / sqrt(1.0 - pow(a.b2, t))),
+                           static_cast<float>(1.0 - lr * a.decay),
+                           __uint_as_float(step_key(a.seed, static_cast<uint64_t>(step), a.slot[k])));
+}
+
+__global__ void __launch_bounds__(256) adam_decode_kernel(int64_t n, const uint8_t* m8, const uint8_t* v8, const int8_t* e,
+                                                          int half, void* m, void* v) {
+  const int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4, left = n - i;
+  if (left <= 0) return;
+  const Quad<uint8_t> qm = load_quad(m8 + i, left), qv = load_quad(v8 + i, left);
+  const int em = e[i / kBlock8 * 2], ev = e[i / kBlock8 * 2 + 1];
+  Quad<float> fm, fv;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) fm.v[j] = decode_m(qm.v[j], em), fv.v[j] = decode_v(qv.v[j], ev);
+  if (half) {
+    Quad<__bf16> hm, hv;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) hm.v[j] = static_cast<__bf16>(fm.v[j]), hv.v[j] = static_cast<__bf16>(fv.v[j]);
+    store_quad(static_cast<__bf16*>(m) + i, hm, left);
+    store_quad(static_cast<__bf16*>(v) + i, hv, left);
+  } else {
+    store_quad(static_cast<float*>(m) + i, fm, left);
+    store_quad(static_cast<float*>(v) + i, fv, left);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- the norm
+struct NormTensor {
+  const void* g;
+  int64_t n;
+  uint32_t first;
+  int half;
+};
+struct NormLaunch {
+  NormTensor t[kNormPer];
+  double* part;
+  uint32_t chunks;
+  int count;
+};
+constexpr int kNormChunk = 8192;  // elements
+
+// Squares in 64 bits: they neither overflow (fp32's do from 1.8e19 on) nor lose small tensors beside large ones;
+// the conversion and the product cost a third of the time that the bytes take.
+template <typename T> IADMM_DEV double square_sum(const T* g, int64_t at, int64_t n) {
+  Quad<T> q[8];
+#pragma unroll
+  for (int u = 0; u < 8; ++u) {
+    const int64_t i = at + u * 1024 + threadIdx.x * 4;
+    q[u] = load_quad(g + i, n - i);
+  }
+  double s = 0.0;
+#pragma unroll
+  for (int u = 0; u < 8; ++u)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const double d = static_cast<double>(static_cast<float>(q[u].v[j]));
+      s = fma(d, d, s);
+    }
+  return s;
+}
+
+IADMM_DEV double block_sum_f64(double s, double* red) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o, kWave);
+  if (threadIdx.x % kWave == 0) red[threadIdx.x / kWave] = s;
+  __syncthreads();
+  s = red[0];
+  for (unsigned w = 1; w < blockDim.x / kWave; ++w) s += red[w];
+  return s;
+}
+
+__global__ void __launch_bounds__(256) norm_kernel(const NormLaunch a) {
+  __shared__ double red[4];
+  double s = 0.0;
+  for (uint32_t c = blockIdx.x; c < a.chunks; c += gridDim.x) {
+    const NormTensor& t = a.t[find_tensor(a, c)];
+    const int64_t at = static_cast<int64_t>(c - t.first) * kNormChunk;
+    s += t.half ? square_sum(static_cast<const __bf16*>(t.g), at, t.n) : square_sum(static_cast<const float*>(t.g), at, t.n);
+  }
+  s = block_sum_f64(s, red);
+  if (threadIdx.x == 0) a.part[blockIdx.x] = s;
+}
+
+__global__ void __launch_bounds__(1024) norm_end_kernel(const double* part, int count, float* norm) {
+  __shared__ double red[16];
+  double s = 0.0;
+  for (int i = threadIdx.x; i < count; i += 1024) s += part[i];
+  s = block_sum_f64(s, red);
+  if (threadIdx.x == 0) *norm = static_cast<float>(sqrt(s));
+}
+
+template <bool EIGHT, int QUADS> static int launch_adam(AdamLaunch& a, hipStream_t st) {
+  uint64_t blocks = 0;
+  for (int k = 0; k < a.count; ++k) {
+    a.t[k].first = static_cast<uint32_t>(blocks);
+    blocks += (static_cast<uint64_t>(a.t[k].n) + 1024 * QUADS - 1) / (1024 * QUADS);
+  }
+  if (blocks > 0x7FFFFFFFu) return IADMM_E_SIZE;
+  hipLaunchKernelGGL((adam_kernel<EIGHT, QUADS>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, st, a);
+  IADMM_CHECK_LAUNCH();
+  return IADMM_OK;
+}
+
+}  // namespace iadmm
+
+using namespace iadmm;
+
+extern "C" int64_t iadmm_grad_norm_ws_bytes(int64_t count) {
+  if (count <= 0) return 0;
+  return (count + kNormPer - 1) / kNormPer * kNormBlocks * static_cast<int64_t>(sizeof(double));
+}
+
+extern "C" int iadmm_grad_norm(int64_t count, const iadmm_grad_tensor* grads, float* norm, void* ws, int64_t ws_bytes,
+                               void* stream) {
+  if (count < 0 || !norm || (count > 0 && (!grads || !ws)) || ws_bytes < iadmm_grad_norm_ws_bytes(count)) return IADMM_E_ARG;
+  if (!aligned16(ws)) return IADMM_E_ALIGN;
+  for (int64_t i = 0; i < count; ++i) {
+    if (grads[i].n < 0 || (grads[i].n > 0 && !grads[i].g) || (grads[i].dtype != IADMM_F32 && grads[i].dtype != IADMM_BF16))
+      return IADMM_E_ARG;
+    if (grads[i].n > (int64_t{1} << 40)) return IADMM_E_SIZE;
+  }
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  double* part = static_cast<double*>(ws);
+  int parts = 0;
+  NormLaunch a;
+  a.count = 0;
+  uint64_t chunks = 0;
+  for (int64_t i = 0; i < count; ++i) {
+    if (grads[i].n > 0) {
+      a.t[a.count++] = NormTensor{grads[i].g, grads[i].n, static_cast<uint32_t>(chunks), grads[i].dtype == IADMM_BF16};
+      chunks += (static_cast<uint64_t>(grads[i].n) + kNormChunk - 1) / kNormChunk;
+      if (chunks > 0x7FFFFFFFu) return IADMM_E_SIZE;
+    }
+    if (a.count > 0 && (a.count == kNormPer || i == count - 1)) {
+      const int blocks = chunks < kNormBlocks ? static_cast<int>(chunks) : kNormBlocks;
+      a.chunks = static_cast<uint32_t>(chunks);
+      a.part = part + parts;
+      hipLaunchKernelGGL(norm_kernel, dim3(blocks), dim3(256), 0, st, a);
+      IADMM_CHECK_LAUNCH();
+      parts += blocks;
+      a.count = 0;
+      chunks = 0;
+    }
+  }
+  hipLaunchKernelGGL(norm_end_kernel, dim3(1), dim3(1024), 0, st, part, parts, norm);
+  IADMM_CHECK_LAUNCH();
+  return IADMM_OK;
+}
+
+extern "C" int64_t iadmm_adamw_ws_bytes(int64_t count) { return count <= 0 ? 0 : count * static_cast<int64_t>(sizeof(float4)); }
+
+extern "C" int iadmm_adamw_step(int64_t count, const iadmm_adamw_tensor* tensors, int state_bits, double lr, const float* lr_dev,
+                                double beta1, double beta2, double eps, double weight_decay, const float* norm,
+                                double max_norm, uint64_t seed, int64_t* steps_dev, void* ws, int64_t ws_bytes,
+                                void* stream) {
+  const bool eight = state_bits == 8;
+  if (count < 0 || (count > 0 && !tensors) || (!eight && state_bits != 32)) return IADMM_E_ARG;
+  if (!(lr >= 0.0) || !(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0) || !(eps >= 0.0) ||
+      !(weight_decay >= 0.0) || (norm && !(max_norm > 0.0)) || (lr_dev && !steps_dev))
+    return IADMM_E_ARG;
+  if (steps_dev && (!ws || ws_bytes < iadmm_adamw_ws_bytes(count))) return IADMM_E_ARG;
+  if (steps_dev && !aligned16(ws)) return IADMM_E_ALIGN;
+  for (int64_t i = 0; i < count; ++i) {
+    const iadmm_adamw_tensor& t = tensors[i];
+    if (t.n < 0 || t.slot < 0 || (t.n > 0 && (!t.p || !t.g || !t.m || !t.v || (eight && !t.e))) ||
+        (!steps_dev && t.step < 1) || (t.dtype != IADMM_F32 && t.dtype != IADMM_BF16) ||
+        (t.gdtype != IADMM_F32 && t.gdtype != IADMM_BF16))
+      return IADMM_E_ARG;
+    if (t.n > (int64_t{1} << 40)) return IADMM_E_SIZE;
+  }
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  float4* table = static_cast<float4*>(ws);
+  for (int64_t from = 0; from < count; from += kPer) {
+    AdamLaunch a;
+    AdamCount c;
+    const int64_t part = count - from < kPer ? count - from : kPer;
+    a.count = 0;
+    int64_t total = 0;
+    for (int64_t i = from; i < from + part; ++i) {
+      const iadmm_adamw_tensor& t = tensors[i];
+      c.slot[i - from] = t.slot;
+      if (t.n == 0 && !steps_dev) continue;  // (with counts on the device an empty tensor counts too)
+      AdamTensor& d = a.t[a.count++];
+      d.p = t.p, d.g = t.g, d.m = t.m, d.v = t.v, d.e = t.e, d.n = t.n, d.slot = t.slot;
+      d.flags = (t.dtype == IADMM_BF16 ? kHalfP : 0) | (t.gdtype == IADMM_BF16 ? kHalfG : 0);
+      const double k = static_cast<double>(t.step);
+      d.step_size = steps_dev ? 0.0f : static_cast<float>(lr / (1.0 - pow(beta1, k)));
+      d.ibc2 = steps_dev ? 0.0f : static_cast<float>(1.0 / sqrt(1.0 - pow(beta2, k)));
+      d.key = steps_dev ? 0u : step_key(seed, static_cast<uint64_t>(t.step), t.slot);
+      total += t.n;
+    }
+    a.norm = norm, a.max_norm = static_cast<float>(max_norm);
+    a.table = steps_dev ? table + from : nullptr;
+    a.decay = static_cast<float>(1.0 - lr * weight_decay), a.eps = static_cast<float>(eps);
+    a.b1 = static_cast<float>(beta1), a.ob1 = static_cast<float>(1.0 - beta1);
+    a.b2 = static_cast<float>(beta2), a.ob2 = static_cast<float>(1.0 - beta2);
+    if (steps_dev) {
+      c.steps = steps_dev, c.lr = lr_dev, c.lr_host = lr, c.b1 = beta1, c.b2 = beta2, c.decay = weight_decay;
+      c.seed = seed, c.table = table + from, c.count = static_cast<int>(part);
+      hipLaunchKernelGGL(adam_count_kernel, dim3(1), dim3(64), 0, st, c);
+      IADMM_CHECK_LAUNCH();
+    }
+    if (total == 0) continue;
+    const int rc = eight ? launch_adam<true, 4>(a, st) : launch_adam<false, 4>(a, st);
+    if (rc) return rc;
+  }
+  return IADMM_OK;
+}
+
+extern "C" int iadmm_adamw_decode8(int64_t n, const void* m8, const void* v8, const void* e, int dtype, void* m, void* v,
+                                   void* stream) {
+  if (n < 0 || (dtype != IADMM_F32 && dtype != IADMM_BF16)) return IADMM_E_ARG;
+  if (n == 0) return IADMM_OK;
+  if (!m8 || !v8 || !e || !m || !v) return IADMM_E_ARG;
+  if (n > (int64_t{1} << 40)) return IADMM_E_SIZE;
+  const int64_t blocks = (n + 1023) / 1024;
+  hipLaunchKernelGGL(adam_decode_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, static_cast<hipStream_t>(stream), n,
+                     static_cast<const uint8_t*>(m8), static_cast<const uint8_t*>(v8), static_cast<const int8_t*>(e),
+                     dtype == IADMM_BF16, m, v);
+  IADMM_CHECK_LAUNCH();
+  return IADMM_OK;
+}

@@ -33,6 +33,7 @@ def _lib_path():
 LIB_PATH = _lib_path()
 
 i64, f32, vp, cint = ctypes.c_int64, ctypes.c_float, ctypes.c_void_p, ctypes.c_int
+f64, u64 = ctypes.c_double, ctypes.c_uint64
 
 # name -> (restype, argtypes); mirrors include/iadmm.h one for one.
 SIGNATURES = {
@@ -89,6 +90,14 @@ SIGNATURES = {
     "iadmm_kkt_bwd_split": (cint, [i64, i64, i64, i64, vp, vp, vp, vp, vp, vp, f32, vp, vp, vp, vp, vp, vp, vp, i64,
                                    vp]),
     "iadmm_loss_grad_split": (cint, [i64, i64, i64] + [vp] * 14 + [i64, vp]),
+    "iadmm_layer_norm_fwd": (cint, [i64, i64, cint, cint, vp, i64, vp, vp, f32, vp, vp, vp, vp]),
+    "iadmm_layer_norm_bwd_ws_bytes": (i64, [i64, i64, cint]),
+    "iadmm_layer_norm_bwd": (cint, [i64, i64, cint, cint, vp, i64, vp, i64] + [vp] * 7 + [i64, vp]),
+    "iadmm_grad_norm_ws_bytes": (i64, [i64]),
+    "iadmm_grad_norm": (cint, [i64, vp, vp, vp, i64, vp]),
+    "iadmm_adamw_ws_bytes": (i64, [i64]),
+    "iadmm_adamw_step": (cint, [i64, vp, cint, f64, vp, f64, f64, f64, f64, vp, f64, u64, vp, vp, i64, vp]),
+    "iadmm_adamw_decode8": (cint, [i64, vp, vp, vp, cint, vp, vp, vp]),
     "iadmm_probe_mfma_flop": (i64, [i64, i64]),
     "iadmm_probe_mfma": (cint, [i64, i64, vp, vp]),
     "iadmm_probe_copy": (cint, [i64, vp, vp, vp]),

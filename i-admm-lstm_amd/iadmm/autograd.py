@@ -291,3 +291,29 @@ class BmvFn(torch.autograd.Function):
         dM = ops.bger(g, x) if ctx.needs_input_grad[0] else None
         dx = ops.bmv_t(M, g) if ctx.needs_input_grad[1] else None
         return dM, dx
+
+
+# ----------------------------------------------------------------------------- layer norm
+class LayerNormFn(torch.autograd.Function):
+    """ops.layer_norm with ops.layer_norm_bwd as its gradient; saves x and 8 bytes a row."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        y, mean, rstd = ops.layer_norm(x, weight, bias, eps, stats=True)
+        ctx.save_for_backward(x, weight, mean, rstd)
+        ctx.wdtype = bias.dtype if bias is not None else None
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, mean, rstd = ctx.saved_tensors
+        dy = dy if ops.has_rows(dy) else dy.contiguous()  # (an expanded gradient, of a sum's output)
+        dx, dw, db = ops.layer_norm_bwd(dy, x, mean, rstd, weight, need=ctx.needs_input_grad[:3], wdtype=ctx.wdtype)
+        return dx, dw, db, None
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5):
+    """Differentiable :func:`iadmm.ops.layer_norm` over the last dimension (x of any layout: copied where its
+    rows are not contiguous)."""
+    return LayerNormFn.apply(x if ops.has_rows(x) else x.contiguous(), weight, bias, eps)

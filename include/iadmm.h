@@ -357,6 +357,65 @@ int iadmm_loss_grad_split(int64_t B, int64_t n, int64_t m, const float* Q, const
                           float* dy, float* dz, void* ws, int64_t ws_bytes, void* stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Layer norm over the rows of a matrix (the hidden state between two iterations,
+ * models/lstm.py ``layer_norm=True``; csrc/layernorm.hip), forward and gradients.
+ * dtype: the type of x, y, dy, dx; wdtype: the type of w, b, dw, db, IADMM_F32 or dtype itself.
+ *   iadmm_layer_norm_fwd: y[rows,cols] = (x - mean) rstd w + b with rstd = 1 / sqrt(var + eps), the
+ *     variance taken over cols; w and b may be NULL (1 and 0); mean[rows] and rstd[rows] (fp32) are
+ *     written where not NULL.  Rows of x lie ldx >= cols elements apart, y is contiguous; y may be x
+ *     (ldx = cols).  No alignment beyond the element's is needed.
+ *   iadmm_layer_norm_bwd: from dy (rows lddy apart) and the forward's x, mean, rstd:
+ *     dx = rstd (q - mean(q) - xhat mean(q xhat)), q = dy w; dw = sum_rows dy xhat; db = sum_rows dy;
+ *     each may be NULL.  The sums over rows have a fixed order (bitwise reproducible).  ws: caller-owned
+ *     16-B aligned workspace of iadmm_layer_norm_bwd_ws_bytes(rows, cols, dtype) bytes (unused where dw
+ *     and db are NULL).  rows = 0 writes dw = db = 0. */
+enum { IADMM_F32 = 0, IADMM_BF16 = 1, IADMM_F16 = 2 };
+int iadmm_layer_norm_fwd(int64_t rows, int64_t cols, int dtype, int wdtype, const void* x, int64_t ldx,
+                         const void* w, const void* b, float eps, void* y, float* mean, float* rstd,
+                         void* stream);
+int64_t iadmm_layer_norm_bwd_ws_bytes(int64_t rows, int64_t cols, int dtype);
+int iadmm_layer_norm_bwd(int64_t rows, int64_t cols, int dtype, int wdtype, const void* dy, int64_t lddy,
+                         const void* x, int64_t ldx, const float* mean, const float* rstd, const void* w,
+                         void* dx, void* dw, void* db, void* ws, int64_t ws_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * The optimizer's step (main.py:350 ``optimizer.step()``) over many tensors at once, and the norm of
+ * all gradients that clipping goes by (csrc/adamw.hip).  The tensor lists are HOST arrays, read during
+ * the call; the pointers in them are device pointers to contiguous tensors (element alignment).
+ *   iadmm_grad_norm: *norm = sqrt(sum over all tensors of g^2), summed in 64 bits in a fixed order.
+ *     ws: iadmm_grad_norm_ws_bytes(count) bytes, 16-B aligned.
+ *   iadmm_adamw_step: for every tensor, in place,
+ *       g' = g min(1, max_norm / (*norm + 1e-6))  (norm NULL: g' = g)
+ *       m = beta1 m + (1 - beta1) g' ; v = beta2 v + (1 - beta2) g'^2
+ *       p = p (1 - lr weight_decay) - lr / (1 - beta1^step) m / (sqrt(v / (1 - beta2^step)) + eps)
+ *     state_bits 32: m, v are fp32.  state_bits 8: m, v hold n codes of 8 bits, e holds two int8 exponents
+ *     for each 256 elements (ceil(n / 256) pairs; all zero is a state of zeros); codes are rounded up or
+ *     down at random, as bf16 parameters are, by (seed, step, slot, element).  dtype / gdtype: IADMM_F32
+ *     or IADMM_BF16.  No two tensors of a call may overlap.
+ *     step: the step that this call makes, counted from 1; or, with steps_dev, steps_dev[slot] is raised by
+ *     1 and used (a captured call then counts its replays); lr_dev (needs steps_dev), where not NULL,
+ *     replaces lr.  ws: iadmm_adamw_ws_bytes(count) bytes, 16-B aligned, with steps_dev only.
+ *   iadmm_adamw_decode8: the values of n 8-bit codes, as fp32 or bf16 (both hold them exactly down to
+ *     2^-126; a moment that overflowed is NaN for m, infinity for v). */
+typedef struct { const void* g; int64_t n; int64_t dtype; } iadmm_grad_tensor;
+typedef struct {
+  void* p; const void* g; void* m; void* v; void* e;
+  int64_t n, step;
+  int32_t slot;            /* the tensor's place: index into steps_dev, part of the random bits */
+  int16_t dtype, gdtype;
+} iadmm_adamw_tensor;
+int64_t iadmm_grad_norm_ws_bytes(int64_t count);
+int iadmm_grad_norm(int64_t count, const iadmm_grad_tensor* grads, float* norm, void* ws, int64_t ws_bytes,
+                    void* stream);
+int64_t iadmm_adamw_ws_bytes(int64_t count);
+int iadmm_adamw_step(int64_t count, const iadmm_adamw_tensor* tensors, int state_bits, double lr,
+                     const float* lr_dev, double beta1, double beta2, double eps, double weight_decay,
+                     const float* norm, double max_norm, uint64_t seed, int64_t* steps_dev, void* ws,
+                     int64_t ws_bytes, void* stream);
+int iadmm_adamw_decode8(int64_t n, const void* m8, const void* v8, const void* e, int dtype, void* m, void* v,
+                        void* stream);
+
+/* ------------------------------------------------------------------------------------------
  * Box-ceiling probes (bench.py roofline.box_ceiling; not on the solve path).
  *   iadmm_probe_mfma: ``blocks`` 256-thread workgroups, each wave issuing ``iters`` x 8
  *     v_mfma_f32_32x32x2_f32 from registers; iadmm_probe_mfma_flop(blocks, iters) flop in all;
