@@ -70,9 +70,10 @@ __host__ __device__ inline uint32_t step_key(uint64_t seed, uint64_t step, int s
 
 // Four neighbouring elements, at any address that the type may have; what lies behind the end is 0.
 template <typename T> struct Quad { T v[4]; };
-template <typename T> IADMM_DEV Quad<T> load_quad(const T* p, int64_t left) {
+// FULL: none lies behind (a branch at each load would keep them from being in flight together).
+template <bool FULL = false, typename T> IADMM_DEV Quad<T> load_quad(const T* p, int64_t left) {
   Quad<T> r;
-  if (left >= 4) {
+  if (FULL || left >= 4) {
     __builtin_memcpy(&r, p, sizeof(r));
   } else {
 #pragma unroll
@@ -80,8 +81,8 @@ template <typename T> IADMM_DEV Quad<T> load_quad(const T* p, int64_t left) {
   }
   return r;
 }
-template <typename T> IADMM_DEV void store_quad(T* p, const Quad<T>& r, int64_t left) {
-  if (left >= 4) {
+template <bool FULL = false, typename T> IADMM_DEV void store_quad(T* p, const Quad<T>& r, int64_t left) {
+  if (FULL || left >= 4) {
     __builtin_memcpy(p, &r, sizeof(r));
   } else {
 #pragma unroll
@@ -117,13 +118,50 @@ IADMM_DEV int block_exponent(uint32_t top, int shift, int low, int high) {
   const int e = static_cast<int>((top + 0x200000u) >> 23) - 127 - shift;
   return e < low ? low : (e > high ? high : e);
 }
+// The largest of the wave's values, as a scalar: six maxima whose second operand comes from another lane (within
+// rows of 16, then across them) instead of twelve instructions through LDS.
+template <int CTRL> IADMM_DEV uint32_t umax_from(uint32_t v) {
+  const uint32_t w = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, 0xF, 0xF, false));
+  return w > v ? w : v;
+}
 IADMM_DEV uint32_t wave_umax(uint32_t v) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) {
-    const uint32_t w = static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), o, kWave));
-    v = w > v ? w : v;
-  }
-  return v;
+  v = umax_from<0x111>(v);  // row_shr 1, 2, 4, 8: lane 15 of each row has its row's
+  v = umax_from<0x112>(v);
+  v = umax_from<0x114>(v);
+  v = umax_from<0x118>(v);
+  v = umax_from<0x142>(v);  // row_bcast 15, 31: lane 63 has the wave's
+  v = umax_from<0x143>(v);
+  return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), 63));
+}
+
+// Four codes at once, as the dword that they lie in.  The scales are products here, so the exponents have to
+// leave 2^(e + 120) and its like normal: kFastM and kFastV, gradients below 10^4 or so; the others, and what is
+// not finite, take the functions above.
+constexpr int kFastM = 6, kFastV = 30;
+IADMM_DEV float pow2(int e) { return bits_f(static_cast<uint32_t>(e + 127) << 23); }  // -126 <= e <= 127
+IADMM_DEV bool ordinary_codes(uint32_t m, uint32_t v) {  // no NaN (m & 127 = 127), no infinity (v = 255)
+  const uint32_t a = (m & 0x7F7F7F7Fu) + 0x01010101u, b = ((v & 0x7F7F7F7Fu) + 0x01010101u) & v;
+  return ((a | b) & 0x80808080u) == 0u;
+}
+template <int J> IADMM_DEV float decode_m_of(uint32_t q, float scale) {
+  const uint32_t mag = J < 3 ? q << (20 - 8 * J) : q >> 4, sign = q << (24 - 8 * J);
+  return bits_f((__float_as_uint(bits_f(mag & 0x07F00000u) * scale) & 0x7FFFFFFFu) | (sign & 0x80000000u));
+}
+template <int J> IADMM_DEV float decode_v_of(uint32_t q, float scale) {
+  return bits_f((J < 3 ? q << (20 - 8 * J) : q >> 4) & 0x0FF00000u) * scale;
+}
+// The code in the top byte.
+IADMM_DEV uint32_t encode_m_top(float m, float scale, uint32_t bits) {
+  const uint32_t a = (__float_as_uint(fabsf(m) * scale) + (bits >> 20 << 8)) << 4;
+  return (a & 0x7FFFFFFFu) | (__float_as_uint(m) & 0x80000000u);
+}
+IADMM_DEV uint32_t encode_v_top(float v, float scale, uint32_t bits) {
+  const uint32_t a = __float_as_uint(v * scale) + (bits & 0xFFFFFu), b = __float_as_uint(v), one = (b < 1u ? b : 1u) << 20;
+  return (a > one ? a : one) << 4;
+}
+IADMM_DEV uint32_t top_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  const uint32_t lo = __builtin_amdgcn_perm(b, a, 0x00000703u), hi = __builtin_amdgcn_perm(d, c, 0x07030000u);
+  return __builtin_amdgcn_perm(hi, lo, 0x07060100u);
 }
 
 // Which of the launch's tensors this workgroup serves: the last whose first workgroup is not behind it.
@@ -146,11 +184,10 @@ struct AdamScalars {
 };
 
 // QUADS x 256 elements per wave, a workgroup's four waves beside each other.
-template <typename P, typename G, bool EIGHT, int QUADS>
-IADMM_DEV void adam_chunk(const AdamLaunch& a, const AdamTensor& t, const AdamScalars& s) {
+template <typename P, typename G, bool EIGHT, int QUADS, bool FULL>
+IADMM_DEV void adam_wave(const AdamLaunch& a, const AdamTensor& t, const AdamScalars& s, int64_t at) {
   using S = typename std::conditional<EIGHT, uint8_t, float>::type;
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  const int64_t at = (static_cast<int64_t>(blockIdx.x - t.first) * 4 + wave) * (QUADS * 256);
+  const int lane = threadIdx.x % kWave;
   P* p = static_cast<P*>(t.p);
   const G* g = static_cast<const G*>(t.g);
   S *m = static_cast<S*>(t.m), *v = static_cast<S*>(t.v);
@@ -162,65 +199,107 @@ IADMM_DEV void adam_chunk(const AdamLaunch& a, const AdamTensor& t, const AdamSc
 #pragma unroll
   for (int u = 0; u < QUADS; ++u) {
     const int64_t i = at + u * 256 + lane * 4, left = t.n - i;
-    qp[u] = load_quad(p + i, left);
-    qg[u] = load_quad(g + i, left);
-    qm[u] = load_quad(m + i, left);
-    qv[u] = load_quad(v + i, left);
+    qp[u] = load_quad<FULL>(p + i, left);
+    qg[u] = load_quad<FULL>(g + i, left);
+    qm[u] = load_quad<FULL>(m + i, left);
+    qv[u] = load_quad<FULL>(v + i, left);
     em[u] = ev[u] = 0;
-    if (EIGHT && at + u * 256 < t.n) {
+    if (EIGHT && (FULL || at + u * 256 < t.n)) {
       em[u] = e[(at + u * 256) / kBlock8 * 2];
       ev[u] = e[(at + u * 256) / kBlock8 * 2 + 1];
     }
   }
 #pragma unroll
   for (int u = 0; u < QUADS; ++u) {
-    if (at + u * 256 >= t.n) break;  // (the whole wave)
+    if (!FULL && at + u * 256 >= t.n) break;  // (the whole wave)
     const int64_t i = at + u * 256 + lane * 4, left = t.n - i;
-    float fm[4], fv[4];
+    float fm[4], fv[4], np[4];
     uint32_t bits[4] = {0, 0, 0, 0};
+    const uint32_t place = static_cast<uint32_t>(i) + static_cast<uint32_t>(i >> 32) * 0x9E3779B9u;  // (i % 4 = 0: no carry)
+    if constexpr (EIGHT) {
+      uint32_t cm, cv;
+      __builtin_memcpy(&cm, &qm[u], 4);
+      __builtin_memcpy(&cv, &qv[u], 4);
+      if (em[u] <= kFastM && ev[u] <= kFastV && __all(ordinary_codes(cm, cv))) {
+        const float sm = pow2(em[u] + 120), sv = pow2(ev[u] + 96);
+        fm[0] = decode_m_of<0>(cm, sm), fm[1] = decode_m_of<1>(cm, sm);
+        fm[2] = decode_m_of<2>(cm, sm), fm[3] = decode_m_of<3>(cm, sm);
+        fv[0] = decode_v_of<0>(cv, sv), fv[1] = decode_v_of<1>(cv, sv);
+        fv[2] = decode_v_of<2>(cv, sv), fv[3] = decode_v_of<3>(cv, sv);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) fm[j] = decode_m(cm >> 8 * j & 255u, em[u]), fv[j] = decode_v(cv >> 8 * j & 255u, ev[u]);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) fm[j] = qm[u].v[j], fv[j] = qv[u].v[j];
+    }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       float gr = static_cast<float>(qg[u].v[j]);
       if (s.clipped) gr = gr * s.clip;
-      float om, ov;
+      fm[j] = a.b1 * fm[j] + a.ob1 * gr;
+      fv[j] = a.b2 * fv[j] + a.ob2 * (gr * gr);
+      const float old = static_cast<float>(qp[u].v[j]) * s.decay;
       if constexpr (EIGHT) {
-        om = decode_m(qm[u].v[j], em[u]);
-        ov = decode_v(qv[u].v[j], ev[u]);
+        // the hardware's root and reciprocal, 1 ulp each: with 8-bit moments the arithmetic takes as long as the
+        // memory, and their correctly rounded forms are a third of it
+        const float d = __builtin_amdgcn_sqrtf(fv[j]) * s.ibc2 + a.eps;
+        np[j] = old - s.step_size * (fm[j] * __builtin_amdgcn_rcpf(d));
       } else {
-        om = qm[u].v[j];
-        ov = qv[u].v[j];
+        np[j] = old - s.step_size * (fm[j] / (sqrtf(fv[j]) * s.ibc2 + a.eps));
       }
-      fm[j] = a.b1 * om + a.ob1 * gr;
-      fv[j] = a.b2 * ov + a.ob2 * (gr * gr);
-      const float d = sqrtf(fv[j]) * s.ibc2 + a.eps;
-      const float np = static_cast<float>(qp[u].v[j]) * s.decay - s.step_size * (fm[j] / d);
       if constexpr (EIGHT || sizeof(P) == 2) {
-        const int64_t k = i + j;
-        bits[j] = mix32((static_cast<uint32_t>(k) + static_cast<uint32_t>(k >> 32) * 0x9E3779B9u) ^ s.key);
-      }
-      if constexpr (sizeof(P) == 2) {
-        const uint32_t b = (__float_as_uint(np) + (bits[j] >> 16)) >> 16;
-        const uint16_t h = static_cast<uint16_t>(np != np ? 0x7FC0u : b);
-        __builtin_memcpy(&qp[u].v[j], &h, 2);
-      } else {
-        qp[u].v[j] = np;
+        bits[j] = mix32((place + j) ^ s.key);
       }
     }
-    store_quad(p + i, qp[u], left);
-    if constexpr (EIGHT) {
-      uint32_t tm = 0, tv = 0;  // (elements behind the end are 0)
+    if constexpr (sizeof(P) == 2) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint32_t bm = is_finite(fm[j]) ? __float_as_uint(fabsf(fm[j])) : 0u;
-        const uint32_t bv = is_finite(fv[j]) ? __float_as_uint(fv[j]) : 0u;
+        const uint32_t b = (__float_as_uint(np[j]) + (bits[j] >> 16)) >> 16;
+        const uint16_t h = static_cast<uint16_t>(np[j] != np[j] ? 0x7FC0u : b);
+        __builtin_memcpy(&qp[u].v[j], &h, 2);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) qp[u].v[j] = np[j];
+    }
+    store_quad<FULL>(p + i, qp[u], left);
+    if constexpr (EIGHT) {
+      uint32_t tm = 0, tv = 0;  // (elements behind the end are 0; v is never negative)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t bm = __float_as_uint(fm[j]) & 0x7FFFFFFFu, bv = __float_as_uint(fv[j]);
         tm = bm > tm ? bm : tm;
         tv = bv > tv ? bv : tv;
       }
-      const int ne = block_exponent(wave_umax(tm), 8, -117, 120), nv = block_exponent(wave_umax(tv), 0, -93, 127);
+      tm = wave_umax(tm);
+      tv = wave_umax(tv);
+      int ne = block_exponent(tm, 8, -117, 120), nv = block_exponent(tv, 0, -93, 127);
+      if (tm < 0x7F800000u && tv < 0x7F800000u && ne <= kFastM && nv <= kFastV) {
+        const float sm = pow2(-ne - 120), sv = pow2(-nv - 96);
+        uint32_t cm[4], cv[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        qm[u].v[j] = static_cast<uint8_t>(encode_m(fm[j], ne, bits[j]));
-        qv[u].v[j] = static_cast<uint8_t>(encode_v(fv[j], nv, bits[j]));
+        for (int j = 0; j < 4; ++j) cm[j] = encode_m_top(fm[j], sm, bits[j]), cv[j] = encode_v_top(fv[j], sv, bits[j]);
+        const uint32_t pm = top_bytes(cm[0], cm[1], cm[2], cm[3]), pv = top_bytes(cv[0], cv[1], cv[2], cv[3]);
+        __builtin_memcpy(&qm[u], &pm, 4);
+        __builtin_memcpy(&qv[u], &pv, 4);
+      } else {  // the exponents are the finite values'
+        tm = tv = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t bm = is_finite(fm[j]) ? __float_as_uint(fabsf(fm[j])) : 0u;
+          const uint32_t bv = is_finite(fv[j]) ? __float_as_uint(fv[j]) : 0u;
+          tm = bm > tm ? bm : tm;
+          tv = bv > tv ? bv : tv;
+        }
+        ne = block_exponent(wave_umax(tm), 8, -117, 120);
+        nv = block_exponent(wave_umax(tv), 0, -93, 127);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          qm[u].v[j] = static_cast<uint8_t>(encode_m(fm[j], ne, bits[j]));
+          qv[u].v[j] = static_cast<uint8_t>(encode_v(fv[j], nv, bits[j]));
+        }
       }
       if (lane == 0) {
         e[(at + u * 256) / kBlock8 * 2] = static_cast<int8_t>(ne);
@@ -230,8 +309,20 @@ IADMM_DEV void adam_chunk(const AdamLaunch& a, const AdamTensor& t, const AdamSc
 #pragma unroll
       for (int j = 0; j < 4; ++j) qm[u].v[j] = fm[j], qv[u].v[j] = fv[j];
     }
-    store_quad(m + i, qm[u], left);
-    store_quad(v + i, qv[u], left);
+    store_quad<FULL>(m + i, qm[u], left);
+    store_quad<FULL>(v + i, qv[u], left);
+  }
+}
+
+template <typename P, typename G, bool EIGHT, int QUADS>
+IADMM_DEV void adam_chunk(const AdamLaunch& a, const AdamTensor& t, const AdamScalars& s) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int64_t at = (static_cast<int64_t>(blockIdx.x - t.first) * 4 + wave) * (QUADS * 256);
+  if (at + QUADS * 256 <= t.n) {
+    adam_wave<P, G, EIGHT, QUADS, true>(a, t, s, at);
+  } else {
+    for (int u = 0; u < QUADS; ++u)
+      if (at + u * 256 < t.n) adam_wave<P, G, EIGHT, 1, false>(a, t, s, at + u * 256);
   }
 }
 
@@ -280,24 +371,41 @@ __global__ void adam_count_kernel(const AdamCount a) {
                            __uint_as_float(step_key(a.seed, static_cast<uint64_t>(step), a.slot[k])));
 }
 
-__global__ void __launch_bounds__(256) adam_decode_kernel(int64_t n, const uint8_t* m8, const uint8_t* v8, const int8_t* e,
-                                                          int half, void* m, void* v) {
-  const int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4, left = n - i;
-  if (left <= 0) return;
-  const Quad<uint8_t> qm = load_quad(m8 + i, left), qv = load_quad(v8 + i, left);
-  const int em = e[i / kBlock8 * 2], ev = e[i / kBlock8 * 2 + 1];
-  Quad<float> fm, fv;
+// The codes' values, 1024 per wave.
+template <typename T, int QUADS, bool FULL> IADMM_DEV void decode_wave(int64_t n, const uint8_t* m8, const uint8_t* v8,
+                                                                       const int8_t* e, T* m, T* v, int64_t at) {
+  const int lane = threadIdx.x % kWave;
+  Quad<uint8_t> qm[QUADS], qv[QUADS];
+  int em[QUADS], ev[QUADS];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) fm.v[j] = decode_m(qm.v[j], em), fv.v[j] = decode_v(qv.v[j], ev);
-  if (half) {
-    Quad<__bf16> hm, hv;
+  for (int u = 0; u < QUADS; ++u) {
+    const int64_t i = at + u * 256 + lane * 4;
+    qm[u] = load_quad<FULL>(m8 + i, n - i);
+    qv[u] = load_quad<FULL>(v8 + i, n - i);
+    em[u] = e[(at + u * 256) / kBlock8 * 2], ev[u] = e[(at + u * 256) / kBlock8 * 2 + 1];
+  }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) hm.v[j] = static_cast<__bf16>(fm.v[j]), hv.v[j] = static_cast<__bf16>(fv.v[j]);
-    store_quad(static_cast<__bf16*>(m) + i, hm, left);
-    store_quad(static_cast<__bf16*>(v) + i, hv, left);
+  for (int u = 0; u < QUADS; ++u) {
+    const int64_t i = at + u * 256 + lane * 4;
+    Quad<T> om, ov;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      om.v[j] = static_cast<T>(decode_m(qm[u].v[j], em[u]));
+      ov.v[j] = static_cast<T>(decode_v(qv[u].v[j], ev[u]));
+    }
+    store_quad<FULL>(m + i, om, n - i);
+    store_quad<FULL>(v + i, ov, n - i);
+  }
+}
+template <typename T> __global__ void __launch_bounds__(256) adam_decode_kernel(int64_t n, const uint8_t* m8, const uint8_t* v8,
+                                                                                const int8_t* e, T* m, T* v) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int64_t at = (static_cast<int64_t>(blockIdx.x) * 4 + wave) * 1024;
+  if (at + 1024 <= n) {
+    decode_wave<T, 4, true>(n, m8, v8, e, m, v, at);
   } else {
-    store_quad(static_cast<float*>(m) + i, fm, left);
-    store_quad(static_cast<float*>(v) + i, fv, left);
+    for (int u = 0; u < 4; ++u)
+      if (at + u * 256 < n) decode_wave<T, 1, false>(n, m8, v8, e, m, v, at + u * 256);
   }
 }
 
@@ -318,12 +426,12 @@ constexpr int kNormChunk = 8192;  // elements
 
 // Squares in 64 bits: they neither overflow (fp32's do from 1.8e19 on) nor lose small tensors beside large ones;
 // the conversion and the product cost a third of the time that the bytes take.
-template <typename T> IADMM_DEV double square_sum(const T* g, int64_t at, int64_t n) {
+template <typename T, bool FULL> IADMM_DEV double square_sum_of(const T* g, int64_t at, int64_t n) {
   Quad<T> q[8];
 #pragma unroll
   for (int u = 0; u < 8; ++u) {
     const int64_t i = at + u * 1024 + threadIdx.x * 4;
-    q[u] = load_quad(g + i, n - i);
+    q[u] = load_quad<FULL>(g + i, n - i);
   }
   double s = 0.0;
 #pragma unroll
@@ -334,6 +442,10 @@ template <typename T> IADMM_DEV double square_sum(const T* g, int64_t at, int64_
       s = fma(d, d, s);
     }
   return s;
+}
+template <typename T> IADMM_DEV double square_sum(const void* g, int64_t at, int64_t n) {
+  const T* p = static_cast<const T*>(g);
+  return at + kNormChunk <= n ? square_sum_of<T, true>(p, at, n) : square_sum_of<T, false>(p, at, n);
 }
 
 IADMM_DEV double block_sum_f64(double s, double* red) {
@@ -348,11 +460,16 @@ IADMM_DEV double block_sum_f64(double s, double* red) {
 
 __global__ void __launch_bounds__(256) norm_kernel(const NormLaunch a) {
   __shared__ double red[4];
+  // a run of neighbouring chunks, so that the tensor is looked for once
+  uint32_t c = static_cast<uint32_t>(static_cast<uint64_t>(a.chunks) * blockIdx.x / gridDim.x);
+  const uint32_t end = static_cast<uint32_t>(static_cast<uint64_t>(a.chunks) * (blockIdx.x + 1) / gridDim.x);
+  int k = find_tensor(a, c);
   double s = 0.0;
-  for (uint32_t c = blockIdx.x; c < a.chunks; c += gridDim.x) {
-    const NormTensor& t = a.t[find_tensor(a, c)];
+  for (; c < end; ++c) {
+    while (k + 1 < a.count && a.t[k + 1].first <= c) ++k;
+    const NormTensor& t = a.t[k];
     const int64_t at = static_cast<int64_t>(c - t.first) * kNormChunk;
-    s += t.half ? square_sum(static_cast<const __bf16*>(t.g), at, t.n) : square_sum(static_cast<const float*>(t.g), at, t.n);
+    s += t.half ? square_sum<__bf16>(t.g, at, t.n) : square_sum<float>(t.g, at, t.n);
   }
   s = block_sum_f64(s, red);
   if (threadIdx.x == 0) a.part[blockIdx.x] = s;
@@ -372,7 +489,7 @@ template <bool EIGHT, int QUADS> static int launch_adam(AdamLaunch& a, hipStream
     a.t[k].first = static_cast<uint32_t>(blocks);
     blocks += (static_cast<uint64_t>(a.t[k].n) + 1024 * QUADS - 1) / (1024 * QUADS);
   }
-  if (blocks > 0x7FFFFFFFu) return IADMM_E_SIZE;
+  if (blocks > 0xFFFFFFu) return IADMM_E_SIZE;  // 2^32 threads
   hipLaunchKernelGGL((adam_kernel<EIGHT, QUADS>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, st, a);
   IADMM_CHECK_LAUNCH();
   return IADMM_OK;
@@ -489,11 +606,17 @@ extern "C" int iadmm_adamw_decode8(int64_t n, const void* m8, const void* v8, co
   if (n < 0 || (dtype != IADMM_F32 && dtype != IADMM_BF16)) return IADMM_E_ARG;
   if (n == 0) return IADMM_OK;
   if (!m8 || !v8 || !e || !m || !v) return IADMM_E_ARG;
-  if (n > (int64_t{1} << 40)) return IADMM_E_SIZE;
-  const int64_t blocks = (n + 1023) / 1024;
-  hipLaunchKernelGGL(adam_decode_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, static_cast<hipStream_t>(stream), n,
-                     static_cast<const uint8_t*>(m8), static_cast<const uint8_t*>(v8), static_cast<const int8_t*>(e),
-                     dtype == IADMM_BF16, m, v);
+  if ((n + 4095) / 4096 > 0xFFFFFF) return IADMM_E_SIZE;  // 2^32 threads
+  const dim3 grid(static_cast<unsigned>((n + 4095) / 4096));
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const uint8_t *cm = static_cast<const uint8_t*>(m8), *cv = static_cast<const uint8_t*>(v8);
+  const int8_t* ex = static_cast<const int8_t*>(e);
+  if (dtype == IADMM_BF16)
+    hipLaunchKernelGGL((adam_decode_kernel<__bf16>), grid, dim3(256), 0, st, n, cm, cv, ex, static_cast<__bf16*>(m),
+                       static_cast<__bf16*>(v));
+  else
+    hipLaunchKernelGGL((adam_decode_kernel<float>), grid, dim3(256), 0, st, n, cm, cv, ex, static_cast<float*>(m),
+                       static_cast<float*>(v));
   IADMM_CHECK_LAUNCH();
   return IADMM_OK;
 }

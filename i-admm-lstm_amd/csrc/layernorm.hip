@@ -8,29 +8,79 @@
 // would cancel for rows whose mean is large against their spread.
 //
 // Bound: HBM.  Forward 2 e bytes an element, backward 3 e (e = element size), ~8 and ~14 flop an element.  So
-// a row is read once and stays in registers: TPR threads hold it, up to 16 elements each, in 16-byte vectors
-// (TPR = 16, 64, 256, 1024 for rows up to 256 / 1024 / 4096 / 16384 elements); longer rows are read again,
-// from L2 for the most part.
+// a row is read once and stays in registers, as the 16-byte vectors that it came in: TPR threads hold it (16,
+// 64, 256 or 1024; row_threads_fwd / row_threads_bwd), longer rows are read again, from L2 for the most part.
+#include <type_traits>
+
 #include "common.h"
 
 namespace iadmm {
 
-typedef unsigned uint4v __attribute__((ext_vector_type(4)));
+// 16 bytes of T in four words (elements of 16 bits as members would take a register each).
+template <typename T> struct Pack {
+  static constexpr int n = 16 / sizeof(T);
+  uint32_t w[4];
+};
+template <typename T> IADMM_DEV float get(const Pack<T>& p, int j) {
+  if constexpr (sizeof(T) == 4) {
+    return __uint_as_float(p.w[j]);
+  } else if constexpr (std::is_same<T, __bf16>::value) {
+    return __uint_as_float(j & 1 ? p.w[j / 2] & 0xFFFF0000u : p.w[j / 2] << 16);
+  } else {
+    const uint16_t b = static_cast<uint16_t>(j & 1 ? p.w[j / 2] >> 16 : p.w[j / 2]);
+    return static_cast<float>(__builtin_bit_cast(_Float16, b));
+  }
+}
+template <typename T> IADMM_DEV void set(Pack<T>& p, const float (&v)[Pack<T>::n]) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if constexpr (sizeof(T) == 4) {
+      p.w[k] = __float_as_uint(v[k]);
+    } else {
+      const T t[2] = {static_cast<T>(v[2 * k]), static_cast<T>(v[2 * k + 1])};
+      __builtin_memcpy(&p.w[k], t, 4);
+    }
+  }
+}
 
-template <typename T> struct Pack;  // 16 bytes of T, at any address that T may have
-template <> struct Pack<float> { static constexpr int n = 4; float v[4]; };
-template <> struct Pack<__bf16> { static constexpr int n = 8; __bf16 v[8]; };
-template <> struct Pack<_Float16> { static constexpr int n = 8; _Float16 v[8]; };
+// Rows of odd length start at any multiple of the element size: the memory pipe takes 16-byte accesses there.
+//
+// Where a thread's vector would reach over the row's end (or lies behind it), it takes the row's last 16 bytes
+// instead: every access is whole, and none has a branch of its own, which would keep a row's loads from being in
+// flight together (8192 rows of 4096 bf16: 48 us with branches, 26 without).  The elements that its neighbours
+// hold too are its first `dup`: they count in no sum, and their result is stored twice, with the same bits.
+struct Place {
+  int64_t at;  // column of its first element
+  int dup;
+};
+template <typename T> IADMM_DEV Place place(int64_t c, int64_t cols) {
+  constexpr int V = Pack<T>::n;
+  const int64_t last = cols - V, at = c < last ? c : last;
+  return Place{at, static_cast<int>(c - at)};
+}
+template <typename T> IADMM_DEV Pack<T> load_whole(const T* p) {
+  Pack<T> r;
+  __builtin_memcpy(&r, p, 16);
+  return r;
+}
 
-// n elements from p (n < Pack::n only at a row's end); what lies behind is 0.  Rows of odd length start at
-// any multiple of the element size: the memory pipe takes 16-byte loads there.
+// n elements from p; what lies behind is 0.  For rows shorter than a vector and for the long rows' kernels.
 template <typename T> IADMM_DEV Pack<T> load_pack(const T* p, int64_t n) {
   Pack<T> r;
   if (n >= Pack<T>::n) {
     __builtin_memcpy(&r, p, 16);
   } else {
+    using U = typename std::conditional<sizeof(T) == 4, uint32_t, uint16_t>::type;
+    const U* q = reinterpret_cast<const U*>(p);
 #pragma unroll
-    for (int j = 0; j < Pack<T>::n; ++j) r.v[j] = j < n ? p[j] : static_cast<T>(0.0f);
+    for (int k = 0; k < 4; ++k) {
+      if constexpr (sizeof(T) == 4) {
+        r.w[k] = k < n ? q[k] : 0u;
+      } else {
+        r.w[k] = 2 * k < n ? q[2 * k] : 0u;
+        if (2 * k + 1 < n) r.w[k] |= static_cast<uint32_t>(q[2 * k + 1]) << 16;
+      }
+    }
   }
   return r;
 }
@@ -38,31 +88,35 @@ template <typename T> IADMM_DEV void store_pack(T* p, const Pack<T>& r, int64_t 
   if (n >= Pack<T>::n) {
     __builtin_memcpy(p, &r, 16);
   } else {
+    using U = typename std::conditional<sizeof(T) == 4, uint32_t, uint16_t>::type;
+    U* q = reinterpret_cast<U*>(p);
 #pragma unroll
     for (int j = 0; j < Pack<T>::n; ++j)
-      if (j < n) p[j] = r.v[j];
+      if (j < n) q[j] = static_cast<U>(sizeof(T) == 4 ? r.w[j * sizeof(T) / 4] : r.w[j / 2] >> (j & 1) * 16);
   }
 }
 
-// V weights from column c (0 behind the end), of type T or fp32; `none` where there are none.
-template <typename T> IADMM_DEV void load_weights(const void* w, bool f32, int64_t c, int64_t cols, float none,
-                                                  float* out) {
+// V weights from column c, of type T or fp32; `none` where there are none.  WHOLE: all within the row.
+template <typename T, bool WHOLE = false> IADMM_DEV void load_weights(const void* w, bool f32, int64_t c, int64_t cols,
+                                                                      float none, float* out) {
   constexpr int V = Pack<T>::n;
-  const int64_t n = cols - c;
+  const int64_t n = WHOLE ? V : cols - c;
   if (!w) {
 #pragma unroll
     for (int j = 0; j < V; ++j) out[j] = none;
   } else if (sizeof(T) == 4 || f32) {
 #pragma unroll
     for (int k = 0; k < V / 4; ++k) {
-      const Pack<float> a = load_pack(static_cast<const float*>(w) + c + 4 * k, n - 4 * k);
+      const float* p = static_cast<const float*>(w) + c + 4 * k;
+      const Pack<float> a = WHOLE ? load_whole(p) : load_pack(p, n - 4 * k);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) out[4 * k + j] = a.v[j];
+      for (int j = 0; j < 4; ++j) out[4 * k + j] = get(a, j);
     }
   } else {
-    const Pack<T> a = load_pack(static_cast<const T*>(w) + c, n);
+    const T* p = static_cast<const T*>(w) + c;
+    const Pack<T> a = WHOLE ? load_whole(p) : load_pack(p, n);
 #pragma unroll
-    for (int j = 0; j < V; ++j) out[j] = static_cast<float>(a.v[j]);
+    for (int j = 0; j < V; ++j) out[j] = get(a, j);
   }
 }
 
@@ -100,58 +154,64 @@ struct LnFwd {
   int w32;
 };
 
-// One row per TPR threads, NV vectors each.
-template <typename T, int TPR, int NV>
+// One row per TPR threads, NV vectors each; SHORT: rows shorter than a vector (TPR = 16, NV = 1).
+template <typename T, int TPR, int NV, bool SHORT>
 __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) ln_fwd_kernel(LnFwd a) {
   constexpr int V = Pack<T>::n, BLOCK = TPR > 256 ? TPR : 256, R = BLOCK / TPR;
   __shared__ float red[2][BLOCK / kWave];
   const int lane = threadIdx.x % TPR;
   const float inv = 1.0f / static_cast<float>(a.cols);
-  for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * R; row0 < a.rows; row0 += static_cast<int64_t>(gridDim.x) * R) {
-    const int64_t row = row0 + threadIdx.x / TPR;
-    const bool on = row < a.rows;
-    const T* x = static_cast<const T*>(a.x) + (on ? row : 0) * a.ldx;
-    float v[NV * V];
+  // (no loop over rows: the weights would be loaded before it and stay in 2 registers an element)
+  const int64_t row = (static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x) * R + threadIdx.x / TPR;
+  const bool on = row < a.rows;
+  const T* x = static_cast<const T*>(a.x) + (on ? row : 0) * a.ldx;
+  Pack<T> p[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int64_t c = static_cast<int64_t>(i * TPR + lane) * V;
+    p[i] = SHORT ? load_pack(x + c, a.cols - c) : load_whole(x + place<T>(c, a.cols).at);
+  }
+  // whether element j of vector i counts; only the row's last vectors have to ask (the same for all threads)
+  auto sum = [&](auto term) {
     float s[1] = {0.0f};
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int64_t c = static_cast<int64_t>(i * TPR + lane) * V;
-      const Pack<T> p = load_pack(x + c, on ? a.cols - c : 0);
+      if (static_cast<int64_t>(i + 1) * TPR * V > a.cols) {
+        const int64_t left = a.cols - c;
+        const int dup = SHORT ? 0 : place<T>(c, a.cols).dup;
 #pragma unroll
-      for (int j = 0; j < V; ++j) v[i * V + j] = static_cast<float>(p.v[j]);
-    }
+        for (int j = 0; j < V; ++j) s[0] += j >= dup && j < (SHORT ? left : V) ? term(get(p[i], j)) : 0.0f;
+      } else {
 #pragma unroll
-    for (int i = 0; i < NV * V; ++i) s[0] += v[i];
-    row_sum<TPR, 1>(s, red[0]);
-    const float mu = s[0] * inv;
-    s[0] = 0.0f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const int64_t c = static_cast<int64_t>(i * TPR + lane) * V + j;
-        v[i * V + j] = c < a.cols ? v[i * V + j] - mu : 0.0f;
-        s[0] = fmaf(v[i * V + j], v[i * V + j], s[0]);
+        for (int j = 0; j < V; ++j) s[0] += term(get(p[i], j));
       }
-    row_sum<TPR, 1>(s, red[1]);
-    const float r = 1.0f / sqrtf(s[0] * inv + a.eps);
-    if (!on) continue;  // (TPR > 64 has one row per workgroup: nobody is left at a barrier)
-    T* y = static_cast<T*>(a.y) + row * a.cols;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int64_t c = static_cast<int64_t>(i * TPR + lane) * V;
-      if (c >= a.cols) continue;
-      float w[V], b[V];
-      load_weights<T>(a.w, a.w32, c, a.cols, 1.0f, w);
-      load_weights<T>(a.b, a.w32, c, a.cols, 0.0f, b);
-      Pack<T> p;
-#pragma unroll
-      for (int j = 0; j < V; ++j) p.v[j] = static_cast<T>(fmaf(v[i * V + j] * r, w[j], b[j]));
-      store_pack(y + c, p, a.cols - c);
     }
-    if (lane == 0 && a.mean) a.mean[row] = mu;
-    if (lane == 0 && a.rstd) a.rstd[row] = r;
+    return s[0];
+  };
+  float s[1] = {sum([](float v) { return v; })};
+  row_sum<TPR, 1>(s, red[0]);
+  const float mu = s[0] * inv;
+  s[0] = sum([mu](float v) { return (v - mu) * (v - mu); });
+  row_sum<TPR, 1>(s, red[1]);
+  const float r = 1.0f / sqrtf(s[0] * inv + a.eps);
+  if (!on) return;
+  T* y = static_cast<T*>(a.y) + row * a.cols;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int64_t c = static_cast<int64_t>(i * TPR + lane) * V;
+    if (c >= a.cols) continue;
+    const int64_t at = SHORT ? c : place<T>(c, a.cols).at;
+    float w[V], b[V];
+    load_weights<T, !SHORT>(a.w, a.w32, at, a.cols, 1.0f, w);
+    load_weights<T, !SHORT>(a.b, a.w32, at, a.cols, 0.0f, b);
+#pragma unroll
+    for (int j = 0; j < V; ++j) w[j] = fmaf((get(p[i], j) - mu) * r, w[j], b[j]);
+    set(p[i], w);
+    store_pack(y + at, p[i], SHORT ? a.cols - at : V);
   }
+  if (lane == 0 && a.mean) a.mean[row] = mu;
+  if (lane == 0 && a.rstd) a.rstd[row] = r;
 }
 
 // Rows longer than the registers hold: a workgroup reads its row three times.
@@ -166,7 +226,7 @@ template <typename T> __global__ void __launch_bounds__(1024) ln_fwd_long_kernel
     for (int64_t c = static_cast<int64_t>(threadIdx.x) * V; c < a.cols; c += TPR * V) {
       const Pack<T> p = load_pack(x + c, a.cols - c);
 #pragma unroll
-      for (int j = 0; j < V; ++j) s[0] += static_cast<float>(p.v[j]);
+      for (int j = 0; j < V; ++j) s[0] += get(p, j);
     }
     row_sum<TPR, 1>(s, red[0]);
     const float mu = s[0] * inv;
@@ -175,7 +235,7 @@ template <typename T> __global__ void __launch_bounds__(1024) ln_fwd_long_kernel
       const Pack<T> p = load_pack(x + c, a.cols - c);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float d = c + j < a.cols ? static_cast<float>(p.v[j]) - mu : 0.0f;
+        const float d = c + j < a.cols ? get(p, j) - mu : 0.0f;
         s[0] = fmaf(d, d, s[0]);
       }
     }
@@ -187,8 +247,8 @@ template <typename T> __global__ void __launch_bounds__(1024) ln_fwd_long_kernel
       load_weights<T>(a.w, a.w32, c, a.cols, 1.0f, w);
       load_weights<T>(a.b, a.w32, c, a.cols, 0.0f, b);
 #pragma unroll
-      for (int j = 0; j < V; ++j)
-        p.v[j] = static_cast<T>(fmaf((static_cast<float>(p.v[j]) - mu) * r, w[j], b[j]));
+      for (int j = 0; j < V; ++j) w[j] = fmaf((get(p, j) - mu) * r, w[j], b[j]);
+      set(p, w);
       store_pack(y + c, p, a.cols - c);
     }
     if (threadIdx.x == 0 && a.mean) a.mean[row] = mu;
@@ -205,13 +265,14 @@ struct LnBwd {
   int w32;
 };
 
-// A workgroup of 1024 threads takes 1024 / TPR rows at a time, at most one workgroup per CU: dw and db grow in
-// registers over all its rows, meet once in LDS and leave as one slab, which keeps the slabs' traffic small
-// beside the rows' (256 slabs at most).
-template <typename T, int TPR, int NV> __global__ void __launch_bounds__(1024) ln_bwd_kernel(LnBwd a) {
-  constexpr int V = Pack<T>::n, R = 1024 / TPR, E = NV * V;
-  extern __shared__ float lds[];  // [2][cols]
-  __shared__ float red[2][2 * 1024 / kWave];
+// A workgroup of BLOCK threads takes BLOCK / TPR rows at a time, one workgroup per CU at most: dw and db grow in
+// registers over all its rows, meet once in LDS and leave as one slab, which keeps the slabs' traffic small beside
+// the rows' (256 slabs at most).  Up to 64 threads a row there is no barrier among them, and a wave waits for its
+// own rows alone.
+template <typename T, int TPR, int NV, int BLOCK, bool SHORT> __global__ void __launch_bounds__(BLOCK) ln_bwd_kernel(LnBwd a) {
+  constexpr int V = Pack<T>::n, R = BLOCK / TPR, E = NV * V;
+  extern __shared__ float lds[];  // [groups][TPR * E]
+  __shared__ float red[2][2 * BLOCK / kWave];
   const int lane = threadIdx.x % TPR, group = threadIdx.x / TPR;
   const float inv = 1.0f / static_cast<float>(a.cols);
   float dw[E], db[E];
@@ -222,58 +283,77 @@ template <typename T, int TPR, int NV> __global__ void __launch_bounds__(1024) l
        row0 += static_cast<int64_t>(gridDim.x) * R, odd ^= 1) {
     const int64_t row = row0 + group;
     const bool on = row < a.rows;
-    const int64_t at = on ? row : 0, cols = on ? a.cols : 0;
-    const T* x = static_cast<const T*>(a.x) + at * a.ldx;
-    const T* dy = static_cast<const T*>(a.dy) + at * a.lddy;
+    const int64_t from = on ? row : 0;
+    const T* x = static_cast<const T*>(a.x) + from * a.ldx;
+    const T* dy = static_cast<const T*>(a.dy) + from * a.lddy;
+    const void* weights = a.w;
+    asm volatile("" : "+s"(weights));  // read again for every row, from the L1: they would not fit the registers
     Pack<T> px[NV], pd[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int64_t c = static_cast<int64_t>(i * TPR + lane) * V;
-      px[i] = load_pack(x + c, cols - c);
-      pd[i] = load_pack(dy + c, cols - c);
+      if constexpr (SHORT) {
+        px[i] = load_pack(x + c, a.cols - c);
+        pd[i] = load_pack(dy + c, a.cols - c);
+      } else {
+        const int64_t at = place<T>(c, a.cols).at;
+        px[i] = load_whole(x + at);
+        pd[i] = load_whole(dy + at);
+      }
     }
-    // (0 in the groups behind the last row, whose dy is 0 too: nothing of them reaches the sums)
-    const float mu = on ? a.mean[row] : 0.0f, r = on ? a.rstd[row] : 0.0f;
+    const float mu = a.mean[from], r = a.rstd[from];
     float s[2] = {0.0f, 0.0f};
-    // dy is 0 behind the row's end, and so is all that comes of it there.  xh and q are made twice from the
-    // row's 16-byte packs: held as fp32 they spill (128 registers for a workgroup of 1024).
+    // xh and q are made twice from the row's 16-byte packs: as fp32 they would take twice to four times the registers
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
+      const int64_t c = static_cast<int64_t>(i * TPR + lane) * V;
+      const Place to = SHORT ? Place{c, 0} : place<T>(c, a.cols);
       float w[V];
-      load_weights<T>(a.w, a.w32, static_cast<int64_t>(i * TPR + lane) * V, a.cols, 1.0f, w);
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float d = static_cast<float>(pd[i].v[j]), h = (static_cast<float>(px[i].v[j]) - mu) * r;
-        const float q = d * w[j];
+      load_weights<T, !SHORT>(weights, a.w32, to.at, a.cols, 1.0f, w);
+      auto add = [&](int j) {
+        const float d = get(pd[i], j), h = (get(px[i], j) - mu) * r, q = d * w[j];
         s[0] += q;
         s[1] = fmaf(q, h, s[1]);
         dw[i * V + j] = fmaf(d, h, dw[i * V + j]);
         db[i * V + j] += d;
+      };
+      if (static_cast<int64_t>(i + 1) * TPR * V > a.cols || row0 + R > a.rows) {  // (the same for the workgroup)
+        const int64_t left = SHORT ? a.cols - c : V;
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (on && j >= to.dup && j < left) add(j);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) add(j);
       }
     }
     row_sum<TPR, 2>(s, red[odd]);
     if (a.dx && on) {
       const float s0 = s[0] * inv, s1 = s[1] * inv;
       T* dx = static_cast<T*>(a.dx) + row * a.cols;
+      asm volatile("" : "+s"(weights));
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int64_t c = static_cast<int64_t>(i * TPR + lane) * V;
         if (c >= a.cols) continue;
+        const int64_t at = SHORT ? c : place<T>(c, a.cols).at;
         float w[V];
-        load_weights<T>(a.w, a.w32, c, a.cols, 1.0f, w);
+        load_weights<T, !SHORT>(weights, a.w32, at, a.cols, 1.0f, w);
         Pack<T> p;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          const float q = static_cast<float>(pd[i].v[j]) * w[j], h = (static_cast<float>(px[i].v[j]) - mu) * r;
-          p.v[j] = static_cast<T>(r * (q - fmaf(h, s1, s0)));
+          const float q = get(pd[i], j) * w[j], h = (get(px[i], j) - mu) * r;
+          w[j] = r * (q - fmaf(h, s1, s0));
         }
-        store_pack(dx + c, p, a.cols - c);
+        set(p, w);
+        store_pack(dx + at, p, SHORT ? a.cols - at : V);
       }
     }
   }
   if (!a.slab) return;
-  // the groups add their sums in their order (a wave's own groups by shuffles first)
-  constexpr int SHARE = TPR < kWave ? kWave / TPR : 1;
+  // The groups' sums meet in LDS: first those of a wave's own groups by shuffles, then all at once, and each column
+  // adds the groups in their order.  (One group after the other took 16 us for the 16 of 800 columns.)
+  constexpr int SHARE = TPR < kWave ? kWave / TPR : 1, PITCH = TPR * E;
 #pragma unroll
   for (int o = kWave / 2; o >= TPR; o >>= 1)
 #pragma unroll
@@ -281,21 +361,37 @@ template <typename T, int TPR, int NV> __global__ void __launch_bounds__(1024) l
       dw[i] += __shfl_xor(dw[i], o, kWave);
       db[i] += __shfl_xor(db[i], o, kWave);
     }
-  for (int g = 0; g < R; g += SHARE) {
-    if (group == g) {
+  const int cols = static_cast<int>(a.cols);
+  float* out = a.slab + static_cast<int64_t>(blockIdx.x) * 2 * a.cols;
 #pragma unroll
-      for (int i = 0; i < E; ++i) {
-        const int64_t c = static_cast<int64_t>(i / V * TPR + lane) * V + i % V;
-        if (c < a.cols) {
-          lds[c] = g ? lds[c] + dw[i] : dw[i];
-          lds[a.cols + c] = g ? lds[a.cols + c] + db[i] : db[i];
+  for (int half = 0; half < 2; ++half) {
+    if (half) __syncthreads();
+    if (group % SHARE == 0) {
+      float* to = lds + group / SHARE * PITCH;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = (i * TPR + lane) * V;
+        const float* v = (half ? db : dw) + i * V;
+        if (c + V <= cols) {
+#pragma unroll
+          for (int j = 0; j < V; j += 4)
+            *reinterpret_cast<float4*>(to + c + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+        } else if (c < cols) {  // the last vector's own elements
+          const Place p = SHORT ? Place{c, 0} : place<T>(c, cols);
+#pragma unroll
+          for (int j = 0; j < V; ++j)
+            if (j >= p.dup && p.at + j < cols) to[p.at + j] = v[j];
         }
       }
     }
     __syncthreads();
+    for (int c = threadIdx.x; c < cols; c += BLOCK) {
+      float s = lds[c];
+#pragma unroll
+      for (int g = 1; g < R / SHARE; ++g) s += lds[g * PITCH + c];
+      out[half * cols + c] = s;
+    }
   }
-  float* out = a.slab + static_cast<int64_t>(blockIdx.x) * 2 * a.cols;
-  for (int64_t c = threadIdx.x; c < 2 * a.cols; c += 1024) out[c] = lds[c];
 }
 
 // Long rows: dx from two readings of the row, dw and db by columns (ln_bwd_cols_kernel).
@@ -316,9 +412,9 @@ template <typename T> __global__ void __launch_bounds__(1024) ln_bwd_long_kernel
 #pragma unroll
       for (int j = 0; j < V; ++j)
         if (c + j < a.cols) {
-          const float q = static_cast<float>(pd.v[j]) * w[j];
+          const float q = get(pd, j) * w[j];
           s[0] += q;
-          s[1] = fmaf(q, (static_cast<float>(px.v[j]) - mu) * r, s[1]);
+          s[1] = fmaf(q, (get(px, j) - mu) * r, s[1]);
         }
     }
     row_sum<TPR, 2>(s, red[odd]);
@@ -329,9 +425,10 @@ template <typename T> __global__ void __launch_bounds__(1024) ln_bwd_long_kernel
       Pack<T> p;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float q = static_cast<float>(pd.v[j]) * w[j], h = (static_cast<float>(px.v[j]) - mu) * r;
-        p.v[j] = static_cast<T>(r * (q - fmaf(h, s1, s0)));
+        const float q = get(pd, j) * w[j], h = (get(px, j) - mu) * r;
+        w[j] = r * (q - fmaf(h, s1, s0));
       }
+      set(p, w);
       store_pack(dx + c, p, a.cols - c);
     }
   }
@@ -350,8 +447,8 @@ template <typename T> __global__ void __launch_bounds__(256) ln_bwd_cols_kernel(
     const float mu = a.mean[row], r = a.rstd[row];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const float d = static_cast<float>(pd.v[j]);
-      dw[j] = fmaf(d, (static_cast<float>(px.v[j]) - mu) * r, dw[j]);
+      const float d = get(pd, j);
+      dw[j] = fmaf(d, (get(px, j) - mu) * r, dw[j]);
       db[j] += d;
     }
   }
@@ -382,13 +479,21 @@ template <typename W> __global__ void __launch_bounds__(1024) ln_slab_kernel(con
 }
 
 constexpr int kCUs = 256;
-constexpr int64_t kMaxHeld = 16384;  // elements of a row that a workgroup holds
+constexpr int64_t kMaxCols = 1 << 24;  // (ln_slab_kernel's grid has 32 threads a column, of 2^32)
+constexpr int64_t kMaxHeld = 16384;  // elements of a row that a workgroup of the backward kernel holds
 
-// Threads per row: as few as hold it with 16 elements each, since fewer meet without a barrier.
-static int row_threads(int64_t cols, int vec) {
-  if (cols <= 16 * 16) return vec == 8 || cols <= 16 * 8 ? 16 : 64;
-  return cols <= 64 * 16 ? 64 : cols <= 256 * 16 ? 256 : 1024;
+// Threads per row, forward: as few as hold it with 8 vectors each, since fewer meet without a barrier (8192 rows
+// of 4096 bf16 took 42 us with 256 threads a row, 26 with 64).
+static int row_threads_fwd(int64_t cols, int vec) {
+  return cols <= 16 * 2 * vec ? 16 : cols <= 64 * 8 * vec ? 64 : cols <= 256 * 8 * vec ? 256 : 1024;
 }
+// Backward: 16 elements each, beside which the sums of dw and db have room in 128 registers (1024 threads), or 32
+// in 256 (512 threads; 64 would spill).
+static int row_threads_bwd(int64_t cols, int vec) {
+  if (cols <= 16 * 16) return vec == 8 || cols <= 16 * 8 ? 16 : 64;
+  return cols <= 64 * 32 ? 64 : cols <= 256 * 16 ? 256 : 1024;
+}
+static int bwd_block(int64_t cols, int tpr) { return tpr == 64 && cols > 64 * 16 ? 512 : 1024; }
 
 static int64_t bwd_slabs(int64_t rows, int64_t cols, int vec) {
   if (rows <= 0) return 0;
@@ -397,43 +502,46 @@ static int64_t bwd_slabs(int64_t rows, int64_t cols, int vec) {
     const int64_t runs = (4 * kCUs + blocks - 1) / blocks;
     return runs < rows ? runs : rows;
   }
-  const int64_t per = 1024 / row_threads(cols, vec);
+  const int tpr = row_threads_bwd(cols, vec);
+  const int64_t per = bwd_block(cols, tpr) / tpr;
   const int64_t need = (rows + per - 1) / per;
   return need < kCUs ? need : kCUs;
 }
 
-template <typename T, int TPR, int NV> static void launch_fwd(const LnFwd& a, hipStream_t st) {
+template <typename T, int TPR, int NV, bool SHORT = false> static void launch_fwd(const LnFwd& a, hipStream_t st) {
   constexpr int block = TPR > 256 ? TPR : 256, r = block / TPR;
-  const int64_t need = (a.rows + r - 1) / r, most = 1 << 20;
-  hipLaunchKernelGGL((ln_fwd_kernel<T, TPR, NV>), dim3(static_cast<unsigned>(need < most ? need : most)), dim3(block), 0,
-                     st, a);
+  const int64_t need = (a.rows + r - 1) / r, most = 1 << 20;  // (a grid's x is at most 2^32 threads)
+  const dim3 grid(static_cast<unsigned>(need < most ? need : most), static_cast<unsigned>((need + most - 1) / most));
+  hipLaunchKernelGGL((ln_fwd_kernel<T, TPR, NV, SHORT>), grid, dim3(block), 0, st, a);
 }
 
 template <typename T> static void fwd(const LnFwd& a, hipStream_t st) {
-  constexpr int V = Pack<T>::n, M = 16 / V;  // vectors of 16 elements
-  if (a.cols > kMaxHeld) {
+  constexpr int V = Pack<T>::n;
+  const int tpr = row_threads_fwd(a.cols, V);
+  const int64_t nv = (a.cols + static_cast<int64_t>(tpr) * V - 1) / (static_cast<int64_t>(tpr) * V);
+  if (tpr == 16) {
+    if (a.cols < V) launch_fwd<T, 16, 1, true>(a, st); else if (nv <= 1) launch_fwd<T, 16, 1>(a, st); else launch_fwd<T, 16, 2>(a, st);
+  } else if (tpr == 64) {
+    if (nv <= 1) launch_fwd<T, 64, 1>(a, st);
+    else if (nv <= 2) launch_fwd<T, 64, 2>(a, st);
+    else if (nv <= 4) launch_fwd<T, 64, 4>(a, st);
+    else launch_fwd<T, 64, 8>(a, st);
+  } else if (tpr == 256) {
+    if (nv <= 4) launch_fwd<T, 256, 4>(a, st); else launch_fwd<T, 256, 8>(a, st);
+  } else if (nv <= 4) {
+    launch_fwd<T, 1024, 4>(a, st);
+  } else {
     const int64_t most = 1 << 20;
     hipLaunchKernelGGL((ln_fwd_long_kernel<T>), dim3(static_cast<unsigned>(a.rows < most ? a.rows : most)), dim3(1024), 0,
                        st, a);
-    return;
-  }
-  const int tpr = row_threads(a.cols, V);
-  const int64_t nv = (a.cols + static_cast<int64_t>(tpr) * V - 1) / (static_cast<int64_t>(tpr) * V);
-  if (tpr == 16) {
-    if (nv <= 1) launch_fwd<T, 16, 1>(a, st); else launch_fwd<T, 16, 2>(a, st);
-  } else if (tpr == 64) {
-    if (nv <= 1) launch_fwd<T, 64, 1>(a, st); else if (nv <= 2) launch_fwd<T, 64, 2>(a, st); else launch_fwd<T, 64, M>(a, st);
-  } else if (tpr == 256) {
-    if (nv <= M / 2) launch_fwd<T, 256, M / 2>(a, st); else launch_fwd<T, 256, M>(a, st);
-  } else {
-    if (nv <= M / 2) launch_fwd<T, 1024, M / 2>(a, st); else launch_fwd<T, 1024, M>(a, st);
   }
 }
 
-template <typename T, int TPR, int NV> static int launch_bwd(const LnBwd& a, int64_t slabs, hipStream_t st) {
-  const int lds = static_cast<int>(2 * a.cols * sizeof(float));
-  IADMM_ALLOW_LDS((ln_bwd_kernel<T, TPR, NV>), lds + 512);
-  hipLaunchKernelGGL((ln_bwd_kernel<T, TPR, NV>), dim3(static_cast<unsigned>(slabs)), dim3(1024), lds, st, a);
+template <typename T, int TPR, int NV, int BLOCK = 1024, bool SHORT = false> static int launch_bwd(const LnBwd& a, int64_t slabs, hipStream_t st) {
+  constexpr int groups = BLOCK / (TPR < kWave ? kWave : TPR);
+  constexpr int lds = groups * TPR * NV * Pack<T>::n * static_cast<int>(sizeof(float));
+  IADMM_ALLOW_LDS((ln_bwd_kernel<T, TPR, NV, BLOCK, SHORT>), lds + 512);
+  hipLaunchKernelGGL((ln_bwd_kernel<T, TPR, NV, BLOCK, SHORT>), dim3(static_cast<unsigned>(slabs)), dim3(BLOCK), lds, st, a);
   return 0;
 }
 
@@ -451,13 +559,18 @@ template <typename T> static int bwd(const LnBwd& a, int64_t slabs, hipStream_t 
     }
     return 0;
   }
-  const int tpr = row_threads(a.cols, V);
+  const int tpr = row_threads_bwd(a.cols, V);
   const int64_t nv = (a.cols + static_cast<int64_t>(tpr) * V - 1) / (static_cast<int64_t>(tpr) * V);
+  if (a.cols < V) return launch_bwd<T, 16, 1, 1024, true>(a, slabs, st);
   if (tpr == 16) return nv <= 1 ? launch_bwd<T, 16, 1>(a, slabs, st) : launch_bwd<T, 16, 2>(a, slabs, st);
-  if (tpr == 64)
-    return nv <= 1 ? launch_bwd<T, 64, 1>(a, slabs, st)
-                   : nv <= 2 ? launch_bwd<T, 64, 2>(a, slabs, st) : launch_bwd<T, 64, M>(a, slabs, st);
-  if (tpr == 256) return nv <= M / 2 ? launch_bwd<T, 256, M / 2>(a, slabs, st) : launch_bwd<T, 256, M>(a, slabs, st);
+  if (tpr == 64) {
+    if (nv <= 1) return launch_bwd<T, 64, 1>(a, slabs, st);
+    if (nv <= 2) return launch_bwd<T, 64, 2>(a, slabs, st);
+    if constexpr (M == 4)
+      if (nv <= 4) return launch_bwd<T, 64, 4>(a, slabs, st);
+    return launch_bwd<T, 64, 2 * M, 512>(a, slabs, st);
+  }
+  if (tpr == 256) return launch_bwd<T, 256, M>(a, slabs, st);
   return nv <= M / 2 ? launch_bwd<T, 1024, M / 2>(a, slabs, st) : launch_bwd<T, 1024, M>(a, slabs, st);
 }
 
@@ -475,7 +588,7 @@ extern "C" int iadmm_layer_norm_fwd(int64_t rows, int64_t cols, int dtype, int w
   if (rows < 0 || cols <= 0 || bad_types(dtype, wdtype) || !(eps >= 0.0f) || !(eps < __builtin_inff())) return IADMM_E_ARG;
   if (rows == 0) return IADMM_OK;
   if (!x || !y || ldx < cols) return IADMM_E_ARG;
-  if (cols > (int64_t{1} << 31)) return IADMM_E_SIZE;
+  if (cols > kMaxCols) return IADMM_E_SIZE;
   const LnFwd a{rows, cols, ldx, x, w, b, y, mean, rstd, eps, wdtype == IADMM_F32};
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == IADMM_F32) fwd<float>(a, st);
@@ -494,7 +607,7 @@ extern "C" int iadmm_layer_norm_bwd(int64_t rows, int64_t cols, int dtype, int w
                                     const void* x, int64_t ldx, const float* mean, const float* rstd, const void* w,
                                     void* dx, void* dw, void* db, void* ws, int64_t ws_bytes, void* stream) {
   if (rows < 0 || cols <= 0 || bad_types(dtype, wdtype)) return IADMM_E_ARG;
-  if (cols > (int64_t{1} << 31)) return IADMM_E_SIZE;
+  if (cols > kMaxCols) return IADMM_E_SIZE;
   const bool sums = dw || db;
   if (rows > 0 && (!dy || !x || !mean || !rstd || lddy < cols || ldx < cols)) return IADMM_E_ARG;
   if (sums && ws_bytes < iadmm_layer_norm_bwd_ws_bytes(rows, cols, dtype)) return IADMM_E_ARG;

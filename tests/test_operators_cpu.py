@@ -21,7 +21,7 @@ def test_layer_norm_arguments():
     refused("bad argument", f, 4, 8, 0, 0, 16, 7, None, None, 1e-5, 16, None, None, None)      # overlapping rows
     refused("bad argument", f, 4, 8, 0, 0, None, 8, None, None, 1e-5, 16, None, None, None)
     refused("bad argument", f, 4, 8, 0, 0, 16, 8, None, None, float("nan"), 16, None, None, None)
-    refused("size beyond", f, 1, (1 << 31) + 1, 0, 0, 16, 1 << 40, None, None, 1e-5, 16, None, None, None)
+    refused("size beyond", f, 1, (1 << 24) + 1, 0, 0, 16, 1 << 40, None, None, 1e-5, 16, None, None, None)
     _abi.call(f, 0, 8, 0, 0, None, 8, None, None, 1e-5, None, None, None, None)                # no rows: nothing to do
     b = "iadmm_layer_norm_bwd"
     need = _abi.lib().iadmm_layer_norm_bwd_ws_bytes(100, 800, 0)
