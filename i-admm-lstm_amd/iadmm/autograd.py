@@ -14,7 +14,7 @@ from __future__ import annotations
 
 import torch
 
-from . import ops
+from . import _abi, ops
 from .solver import PARAM_NAMES
 
 GATES = "ifou"
@@ -294,26 +294,8 @@ class BmvFn(torch.autograd.Function):
 
 
 # ----------------------------------------------------------------------------- layer norm
-class LayerNormFn(torch.autograd.Function):
-    """ops.layer_norm with ops.layer_norm_bwd as its gradient; saves x and 8 bytes a row."""
-
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps):
-        y, mean, rstd = ops.layer_norm(x, weight, bias, eps, stats=True)
-        ctx.save_for_backward(x, weight, mean, rstd)
-        ctx.wdtype = bias.dtype if bias is not None else None
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        x, weight, mean, rstd = ctx.saved_tensors
-        dy = dy if ops.has_rows(dy) else dy.contiguous()  # (an expanded gradient, of a sum's output)
-        dx, dw, db = ops.layer_norm_bwd(dy, x, mean, rstd, weight, need=ctx.needs_input_grad[:3], wdtype=ctx.wdtype)
-        return dx, dw, db, None
-
-
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """Differentiable :func:`iadmm.ops.layer_norm` over the last dimension (x of any layout: copied where its
-    rows are not contiguous)."""
-    return LayerNormFn.apply(x if ops.has_rows(x) else x.contiguous(), weight, bias, eps)
+    rows are not contiguous); its backward is :func:`iadmm.ops.layer_norm_bwd`.  Saves x and 8 bytes a row.
+    A C++ autograd node (csrc/native.cpp), once differentiable."""
+    return _abi.native().layer_norm_grad(x, weight, bias, eps)

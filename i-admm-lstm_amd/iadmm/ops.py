@@ -4,15 +4,12 @@ Every wrapper takes contiguous fp32 tensors on the current HIP device, allocates
 with the PyTorch caching allocator, launches on the current stream and returns.  There is no
 host synchronisation and no CPU path: a CPU tensor or a missing library raises.  The wrappers of the
 last two sections (layer norm, the optimizer's step) also take bf16 (layer norm: fp16 too), and launch
-on the current stream of their tensors' device, whichever device is current.
+on the current stream of their tensors' device, whichever device is current; their checks and packing
+are csrc/native.cpp's.
 """
 from __future__ import annotations
 
-import array
-import contextlib
 import ctypes
-import itertools
-import math
 import threading
 
 import torch
@@ -550,81 +547,13 @@ def loss_grad(Q, p, A0, x, y, z, cp=None, cd=None, want_grad=True, split=True, w
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # include/iadmm.h IADMM_F32, _BF16, _F16
 
 
-def _on(device):
-    """Makes ``device`` current where it is not (a launch goes to the current device)."""
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-
-def _stream_of(device):
-    return torch.cuda.current_stream(device).cuda_stream
-
-
-def _device_tensor(t, what, device=None):
-    if not t.is_cuda:
-        raise ValueError("iadmm kernels need device tensors (no CPU fallback)")
-    if device is not None and t.device != device:
-        raise ValueError(f"{what} is on {t.device}, not on {device}")
-
-
-def _rows_of(t, what):
-    """(rows, cols, elements from row to row) of a tensor whose last dimension is the row; contiguous, or
-    two-dimensional with contiguous rows that do not overlap."""
-    if t.dim() < 1 or t.shape[-1] == 0:
-        raise ValueError(f"{what} needs a last dimension of at least one element, got {tuple(t.shape)}")
-    cols = t.shape[-1]
-    if t.is_contiguous():
-        return t.numel() // cols, cols, cols
-    if t.dim() == 2 and (t.stride(1) == 1 or cols == 1) and t.stride(0) >= cols:
-        return t.shape[0], cols, t.stride(0)
-    raise ValueError(f"{what} needs contiguous rows, got strides {t.stride()} for {tuple(t.shape)}")
-
-
-def has_rows(t):
-    """Whether :func:`layer_norm` takes ``t`` as it lies in memory."""
-    return t.is_contiguous() or (t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= t.shape[1])
-
-
-def _row_vector(w, x, cols, what):
-    if w is None:
-        return None
-    _device_tensor(w, what, x.device)
-    if w.shape != (cols,) or not w.is_contiguous():
-        raise ValueError(f"{what} must be contiguous [{cols}], got {tuple(w.shape)}")
-    if w.dtype != torch.float32 and w.dtype != x.dtype:
-        raise TypeError(f"{what} must be float32 or {x.dtype}, got {w.dtype}")
-    return w.data_ptr()
-
-
 def layer_norm(x, weight=None, bias=None, eps=1e-5, out=None, stats=False):
     """(x - mean) / sqrt(var + eps) * weight + bias over the last dimension, in x's type (fp32, bf16 or fp16;
     statistics and arithmetic are fp32).  ``weight`` / ``bias``: [cols], fp32 or of x's type, both the same.
     x: contiguous, or 2-D with contiguous rows.  ``out``: contiguous, of x's shape and type; x itself where x
     is contiguous.  ``stats``: returns (y, mean, rstd), the fp32 statistics of each row that
-    :func:`layer_norm_bwd` takes.  The gradient: :func:`iadmm.autograd.layer_norm`."""
-    _device_tensor(x, "x")
-    if x.dtype not in DTYPES:
-        raise TypeError(f"layer_norm computes on {', '.join(str(t) for t in DTYPES)}, got {x.dtype}")
-    if not 0.0 <= eps < math.inf:
-        raise ValueError(f"eps must be finite and not negative, got {eps}")
-    rows, cols, ld = _rows_of(x, "x")
-    w, b = _row_vector(weight, x, cols, "weight"), _row_vector(bias, x, cols, "bias")
-    if w is not None and b is not None and weight.dtype != bias.dtype:
-        raise TypeError(f"weight is {weight.dtype} and bias {bias.dtype}: both must be of one type")
-    if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    else:
-        _device_tensor(out, "out", x.device)
-        if out.shape != x.shape or out.dtype != x.dtype or not out.is_contiguous():
-            raise ValueError(f"out must be contiguous {tuple(x.shape)} {x.dtype}")
-    mean = rstd = None
-    if stats:
-        mean, rstd = torch.empty(2, *x.shape[:-1], dtype=torch.float32, device=x.device).unbind(0)
-    wt = DTYPES[weight.dtype] if w is not None else DTYPES[bias.dtype] if b is not None else 0
-    with _on(x.device):
-        _abi.call("iadmm_layer_norm_fwd", rows, cols, DTYPES[x.dtype], wt, x.data_ptr(), ld, w, b, float(eps),
-                  out.data_ptr(), mean.data_ptr() if stats else None, rstd.data_ptr() if stats else None,
-                  _stream_of(x.device))
-    return (out, mean, rstd) if stats else out
+    :func:`layer_norm_bwd` takes.  No gradient: :func:`iadmm.autograd.layer_norm` has it."""
+    return _abi.native().layer_norm(x, weight, bias, eps, out, stats)
 
 
 def layer_norm_bwd(dy, x, mean, rstd, weight=None, need=(True, True, True), wdtype=None):
@@ -632,80 +561,18 @@ def layer_norm_bwd(dy, x, mean, rstd, weight=None, need=(True, True, True), wdty
     dx has x's type, dweight and dbias weight's (``wdtype`` or fp32 without a weight).  ``need``: which to
     compute (the others are None).  The sums over rows have a fixed order: the same inputs give the same
     bits."""
-    _device_tensor(x, "x")
-    if x.dtype not in DTYPES or dy.dtype != x.dtype:
-        raise TypeError(f"x and dy must be of one type of {', '.join(str(t) for t in DTYPES)}, got {x.dtype}, {dy.dtype}")
-    _device_tensor(dy, "dy", x.device)
-    if dy.shape != x.shape:
-        raise ValueError(f"dy is {tuple(dy.shape)}, x {tuple(x.shape)}")
-    rows, cols, ld = _rows_of(x, "x")
-    _, _, lddy = _rows_of(dy, "dy")
-    for name, t in (("mean", mean), ("rstd", rstd)):
-        _device_tensor(t, name, x.device)
-        if t.dtype != torch.float32 or not t.is_contiguous() or t.numel() != rows:
-            raise ValueError(f"{name} must be contiguous fp32 with {rows} values")
-    w = _row_vector(weight, x, cols, "weight")
-    wdtype = weight.dtype if weight is not None else wdtype or torch.float32
-    if wdtype != torch.float32 and wdtype != x.dtype:
-        raise TypeError(f"wdtype must be float32 or {x.dtype}, got {wdtype}")
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need[0] else None
-    dw = torch.empty(cols, dtype=wdtype, device=x.device) if need[1] else None
-    db = torch.empty(cols, dtype=wdtype, device=x.device) if need[2] else None
-    nbytes, ws = 0, None
-    if need[1] or need[2]:
-        nbytes = int(_abi.lib().iadmm_layer_norm_bwd_ws_bytes(rows, cols, DTYPES[x.dtype]))
-        ws = torch.empty(nbytes // 4, dtype=torch.float32, device=x.device)
-    with _on(x.device):
-        _abi.call("iadmm_layer_norm_bwd", rows, cols, DTYPES[x.dtype], DTYPES[wdtype], dy.data_ptr(), lddy, x.data_ptr(),
-                  ld, mean.data_ptr(), rstd.data_ptr(), w, *(t.data_ptr() if t is not None else None
-                                                             for t in (dx, dw, db, ws)), nbytes, _stream_of(x.device))
-    return dx, dw, db
+    return _abi.native().layer_norm_bwd(dy, x, mean, rstd, weight, DTYPES[wdtype or torch.float32], *need)
 
 
 # --------------------------------------------------------------------------- the optimizer's step
-ADAM_DTYPES = {torch.float32: 0, torch.bfloat16: 1}
 ADAM_BLOCK = 256  # elements that share the exponents of their 8-bit moments
-
-
-def _list_device(ts, what, dtypes):
-    """The device of a list of contiguous tensors of the given types."""
-    kinds = set(map(_TENSOR.dtype.__get__, ts))
-    if not kinds <= dtypes:
-        raise TypeError(f"{what} must be {' or '.join(sorted(str(t) for t in dtypes))}, got {sorted(map(str, kinds))}")
-    devices = set(map(_TENSOR.device.__get__, ts))
-    if len(devices) != 1:
-        raise ValueError(f"{what} must be on one device, got {sorted(map(str, devices))}")
-    if not all(map(_TENSOR.is_contiguous, ts)):
-        raise ValueError(f"{what} must be contiguous")
-    device, = devices
-    if device.type != "cuda":
-        raise ValueError("iadmm kernels need device tensors (no CPU fallback)")
-    return device
-
-
-_TENSOR = torch._C.TensorBase
-_FLOATS = frozenset(ADAM_DTYPES)
-_F32, _U8, _I8 = (frozenset((t,)) for t in (torch.float32, torch.uint8, torch.int8))
 
 
 def grad_norm(grads):
     """The 2-norm of all elements of a list of gradients (contiguous, fp32 or bf16; None is left out) as a
     0-dim fp32 device tensor: what clipping by the global norm goes by.  Summed in 64 bits, in a fixed
     order."""
-    grads = [g for g in grads if g is not None]
-    if not grads:
-        raise ValueError("grad_norm needs at least one gradient")
-    device = _list_device(grads, "gradients", _FLOATS)
-    n = len(grads)
-    rec = array.array("q", itertools.chain.from_iterable(zip(
-        map(_TENSOR.data_ptr, grads), map(_TENSOR.numel, grads), (ADAM_DTYPES[g.dtype] for g in grads))))
-    nbytes = int(_abi.lib().iadmm_grad_norm_ws_bytes(n))
-    buf = torch.empty(nbytes // 4 + 4, dtype=torch.float32, device=device)
-    norm = torch.empty((), dtype=torch.float32, device=device)
-    with _on(device):
-        _abi.call("iadmm_grad_norm", n, rec.buffer_info()[0], norm.data_ptr(), buf.data_ptr(), nbytes,
-                  _stream_of(device))
-    return norm
+    return _abi.native().grad_norm(grads)
 
 
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8,
@@ -727,93 +594,30 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9, 
     min(1, max_norm / (norm + 1e-6)); they themselves stay as they are.
 
     No two tensors of the call may overlap.  A call with an error changes nothing."""
-    count = len(params)
-    eight = exponents is not None
-    if not (count == len(grads) == len(exp_avgs) == len(exp_avg_sqs)) or (eight and len(exponents) != count):
-        raise ValueError("the lists must have one entry per parameter")
-    if (norm is None) != (max_norm is None):
-        raise ValueError("norm and max_norm belong together")
-    lists = [params, grads, exp_avgs, exp_avg_sqs] + ([exponents] if eight else [])
-    slots = range(count)
-    if any(g is None for g in grads):
-        slots = [i for i in slots if grads[i] is not None]
-        lists = [[ts[i] for i in slots] for ts in lists]
-    if not slots:
-        return
-    device = _list_device(lists[0], "params", _FLOATS)
-    kinds = (("params", _FLOATS), ("grads", _FLOATS), ("exp_avgs", _U8 if eight else _F32),
-             ("exp_avg_sqs", _U8 if eight else _F32), ("exponents", _I8))
-    sizes = list(map(_TENSOR.numel, lists[0]))
-    for (what, dtypes), ts in zip(kinds[1:], lists[1:]):
-        if _list_device(ts, what, dtypes) != device:
-            raise ValueError(f"{what} must be on the device of params, {device}")
-        want = sizes if what != "exponents" else [(n + ADAM_BLOCK - 1) // ADAM_BLOCK * 2 for n in sizes]
-        if list(map(_TENSOR.numel, ts)) != want:
-            raise ValueError(f"{what} must match the parameters' sizes")
-    if any(g.shape != p.shape for p, g in zip(lists[0], lists[1])):
-        raise ValueError("a gradient must have its parameter's shape")
-    ptrs = [list(map(_TENSOR.data_ptr, ts)) for ts in lists]
-    held = [q for ps in (ptrs[0], *ptrs[2:]) for q in ps if q]
-    if len(set(held)) != len(held):
-        raise ValueError("a parameter or its state is in the lists twice")
-    lr_dev = steps_dev = ws = None
-    nbytes = 0
-    if isinstance(step, torch.Tensor):
-        _device_tensor(step, "step", device)
-        if step.dtype != torch.int64 or step.shape != (count,) or not step.is_contiguous():
-            raise ValueError(f"step must be contiguous int64 [{count}], got {step.dtype} {tuple(step.shape)}")
-        steps_dev, steps = step.data_ptr(), itertools.repeat(0)
-        nbytes = int(_abi.lib().iadmm_adamw_ws_bytes(len(slots)))
-        ws = torch.empty(nbytes // 4, dtype=torch.float32, device=device)
-        if isinstance(lr, torch.Tensor):
-            _device_tensor(lr, "lr", device)
-            if lr.dtype != torch.float32 or lr.numel() != 1:
-                raise ValueError("a device lr must be one fp32 value")
-            lr_dev, lr = lr.data_ptr(), 0.0
-    else:
-        if isinstance(lr, torch.Tensor):
-            raise TypeError("lr on the device needs step on the device")
-        steps = [int(step)] * len(slots) if not hasattr(step, "__len__") else [int(step[i]) for i in slots]
-        if min(steps) < 1:
-            raise ValueError("steps are counted from 1")
-        if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("a captured step needs its count on the device (an int64 tensor as step): a number "
-                               "would be the same at every replay")
-    if norm is not None:
-        _device_tensor(norm, "norm", device)
-        if norm.dtype != torch.float32 or norm.numel() != 1:
-            raise ValueError("norm must be one fp32 value")
-        if not max_norm > 0:
-            raise ValueError(f"max_norm must be positive, got {max_norm}")
-    if not (0 <= lr < math.inf and 0 <= betas[0] < 1 and 0 <= betas[1] < 1 and 0 <= eps < math.inf and
-            0 <= weight_decay < math.inf):
-        raise ValueError(f"lr {lr}, betas {betas}, eps {eps} or weight_decay {weight_decay} is out of range")
-    # iadmm_adamw_tensor: five pointers, n, step, then slot (32 bits), dtype and gdtype (16 each)
-    kind = (i | ADAM_DTYPES[p.dtype] << 32 | ADAM_DTYPES[g.dtype] << 48 for i, p, g in zip(slots, lists[0], lists[1]))
-    rec = array.array("q", itertools.chain.from_iterable(zip(
-        *ptrs[:4], ptrs[4] if eight else itertools.repeat(0), sizes, steps, kind)))
-    with _on(device):
-        _abi.call("iadmm_adamw_step", len(slots), rec.buffer_info()[0], 8 if eight else 32, lr, lr_dev, betas[0], betas[1],
-                  eps, weight_decay, norm.data_ptr() if norm is not None else None, max_norm or 0.0,
-                  seed & 0xFFFFFFFFFFFFFFFF, steps_dev, ws.data_ptr() if ws is not None else None, nbytes,
-                  _stream_of(device))
-    # the kernel wrote behind autograd's back: whoever goes by the version (solver.PackedWeights) has to see it
-    torch.autograd.graph.increment_version([p for p in lists[0] if not p.is_inference()])
+    if (not isinstance(step, torch.Tensor) and len(params) and getattr(params[0], "is_cuda", False)
+            and torch.cuda.is_current_stream_capturing()):
+        raise RuntimeError("a captured step needs its count on the device (an int64 tensor as step): a number "
+                           "would be the same at every replay")
+    _abi.native().adamw_step(params, grads, exp_avgs, exp_avg_sqs, exponents, step, lr, betas[0], betas[1], eps,
+                             weight_decay, norm, max_norm, seed)
 
 
 def adamw_decode8(exp_avg, exp_avg_sq, exponents, dtype=torch.bfloat16):
     """(m, v): the values that the 8-bit moments of :func:`adamw_step` stand for, as bf16 or fp32 (either holds
     them exactly).  A moment that overflowed is NaN in m, infinity in v."""
-    device = _list_device([exp_avg, exp_avg_sq], "moments", _U8)
-    if _list_device([exponents], "exponents", _I8) != device:
-        raise ValueError(f"exponents must be on {device}")
-    n = exp_avg.numel()
+    device, n = exp_avg.device, exp_avg.numel()
+    for what, t, kind in (("exp_avg", exp_avg, torch.uint8), ("exp_avg_sq", exp_avg_sq, torch.uint8),
+                          ("exponents", exponents, torch.int8)):
+        if t.dtype != kind or not t.is_contiguous():
+            raise TypeError(f"{what} must be contiguous {kind}, got {t.dtype}")
+        if not t.is_cuda or t.device != device:
+            raise ValueError(f"iadmm kernels need device tensors (no CPU fallback) on one device; {what} is on {t.device}")
     if exp_avg_sq.shape != exp_avg.shape or exponents.numel() != (n + ADAM_BLOCK - 1) // ADAM_BLOCK * 2:
         raise ValueError("moments must be of one shape, exponents [ceil(numel / 256), 2]")
-    if dtype not in ADAM_DTYPES:
+    if dtype not in (torch.float32, torch.bfloat16):
         raise TypeError(f"dtype must be float32 or bfloat16, got {dtype}")
     m, v = torch.empty(2, *exp_avg.shape, dtype=dtype, device=device).unbind(0)
-    with _on(device):
+    with torch.cuda.device(device):
         _abi.call("iadmm_adamw_decode8", n, exp_avg.data_ptr(), exp_avg_sq.data_ptr(), exponents.data_ptr(),
-                  ADAM_DTYPES[dtype], m.data_ptr(), v.data_ptr(), _stream_of(device))
+                  DTYPES[dtype], m.data_ptr(), v.data_ptr(), _stream())
     return m, v

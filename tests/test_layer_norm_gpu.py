@@ -242,6 +242,21 @@ def test_frozen_parts_get_no_gradient():
     y = autograd.layer_norm(x.detach(), w.requires_grad_(True), b)
     y.backward(dy)
     assert w.grad is not None and b.grad is None
+    full = torch.autograd.grad(autograd.layer_norm(x, w, b.requires_grad_(True)), (x, w, b), dy)
+    only, = torch.autograd.grad(autograd.layer_norm(x.detach(), None, b), b, dy)
+    assert torch.equal(only, full[2]) and torch.equal(w.grad, full[1]) and not autograd.layer_norm(x.detach()).requires_grad
+    with torch.no_grad():
+        assert not autograd.layer_norm(x, w, b).requires_grad
+
+
+def test_gradient_of_the_gradient_is_refused():
+    from iadmm import autograd
+    x, dy, w, b = inputs(4, 50, F32, F32)
+    x.requires_grad_(True)
+    g, = torch.autograd.grad(autograd.layer_norm(x, w, b), x, dy, create_graph=True)
+    assert bool(torch.isfinite(g).all())
+    with pytest.raises(RuntimeError, match="no gradient of its own"):
+        torch.autograd.grad(g.sum(), x)
 
 
 def test_other_stream_and_replayed_graph():
