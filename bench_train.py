@@ -47,6 +47,10 @@ def main():
     ap.add_argument("--reduce", choices=("ordered", "allreduce"), default="ordered",
                     help="gradient reduction over ranks (iadmm/train.py): the ordered fold (bitwise "
                          "world-size invariant) or the ring all-reduce")
+    ap.add_argument("--optimizer", choices=("adam", "adamw"), default="adam",
+                    help="torch's Adam, or the multi-tensor AdamW of iadmm/optim.py")
+    ap.add_argument("--state_bits", type=int, choices=(8, 32), default=32, help="bits of AdamW's moments")
+    ap.add_argument("--layer_norm", action="store_true", help="normalise the hidden state before the gates' product")
     args = ap.parse_args()
     launch_ranks(args)
     from iadmm import data, ops, parallel, train
@@ -61,8 +65,12 @@ def main():
     Qs, ps, As, zls, zus, _, _, _ = ops.ruiz_scale(d["Q"], d["p"], d["A0"], d["zl"], d["zu"], 10)
     d = dict(Q=Qs, p=ps, A0=As, zl=zls, zu=zus)
     torch.manual_seed(17)
-    model = LSTM(mi + me, 2, h, T, "cuda")
-    opt = torch.optim.Adam(model.parameters(), lr=5e-5)
+    model = LSTM(mi + me, 2, h, T, "cuda", layer_norm=args.layer_norm)
+    if args.optimizer == "adamw":
+        from iadmm.optim import AdamW
+        opt = AdamW(model.parameters(), lr=5e-5, weight_decay=0.0, state_bits=args.state_bits)
+    else:
+        opt = torch.optim.Adam(model.parameters(), lr=5e-5)
 
     def step():
         return train.tbptt_batch(model, d, mi, me, T, T, 6e-6, opt, micro_batch=args.micro_batch,

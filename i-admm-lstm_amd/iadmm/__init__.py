@@ -2,7 +2,8 @@
 
 Layers: ``_abi`` (ctypes binding of libiadmm.so, the C-ABI in include/iadmm.h) -> ``ops``
 (tensor-level kernel wrappers) -> ``solver`` (the fused test-mode solve loop) and
-``kktop`` (the lazy KKT operator returned as ``A_tild``).  The reference-compatible module
+``kktop`` (the lazy KKT operator returned as ``A_tild``); training goes through ``autograd``, ``train`` and
+``optim`` (AdamW).  The reference-compatible module
 surface (models/lstm.py, models/lu.py, methods/scaling.py, utils.py, main.py) lives at the repo
 root and is built on these.
 """

@@ -5,9 +5,10 @@ of instances that is already resident in HBM.  Every step is a HIP kernel from l
 the current stream; no host synchronisation happens inside (metrics are kept on the device and
 copied once at the end when ``history`` is requested).
 
-Per iteration t (4 launches):
+Per iteration t (4 launches, 5 for a model with layer_norm):
   iadmm_schedule      rho/alpha scalars of step t            models/lstm.py:60-63
   iadmm_kkt_resgrad   g = K^T (K xv - b~), implicit K        models/lstm.py:67-72
+  (iadmm_layer_norm_fwd the hidden state's normalisation)
   iadmm_lstm_cell_fwd gates on fp32 MFMA + cell + projection models/lstm.py:74-80
   iadmm_admm_update   xv, x, z, y updates                    models/lstm.py:80-94
 Buffers: x/y/z/xv and H ping-pong between two sets owned by the solver; C is updated in place.
@@ -21,10 +22,16 @@ from . import ops
 PARAM_NAMES = tuple(f"{a}_{g}" for g in "ifou" for a in ("W", "U", "b")) + ("W_h", "b_h", "rho", "alpha")
 
 
+LN_NAMES = ("ln_w", "ln_b")  # of a model with layer_norm: the hidden state's normalisation before the gates' product
+LN_EPS = 1e-5
+
+
 def param_dict(model_or_dict):
-    if isinstance(model_or_dict, dict):
-        return {k: model_or_dict[k] for k in PARAM_NAMES}
-    return {k: getattr(model_or_dict, k) for k in PARAM_NAMES}
+    """The cell's 16 parameters by name, and LN_NAMES of a model (or dict) that has them."""
+    get = model_or_dict.get if isinstance(model_or_dict, dict) else lambda k: getattr(model_or_dict, k, None)
+    d = {k: model_or_dict[k] if isinstance(model_or_dict, dict) else getattr(model_or_dict, k) for k in PARAM_NAMES}
+    d.update({k: get(k) for k in LN_NAMES if get(k) is not None})
+    return d
 
 
 class PackedWeights:
@@ -157,11 +164,17 @@ def solve(params, Q, p, A0, zl, zu, num_ineq, num_eq, T, sigma, scaling=True, sc
     ``precision="f16x3"`` runs the gate GEMM on the fp16 matrix cores with the 3-term split of
     csrc/lstm_f16x3.hip (optional mode; the default "f32" is the fp32-MFMA path): H is carried as
     its two fp16 planes between iterations and the fp32 H is written on the last iteration.
+
+    ``params`` with ``ln_w`` / ``ln_b`` (a model with layer_norm): the gates take the normalised hidden state;
+    fp32 only.
     """
     if precision not in PRECISIONS:
         raise ValueError(f"precision must be one of {PRECISIONS}")
     f16 = precision == "f16x3"
     params = param_dict(params)
+    normed = "ln_w" in params
+    if normed and f16:
+        raise ValueError("a model with layer_norm solves with precision='f32'")
     B, n = Q.shape[0], Q.shape[1]
     m = A0.shape[1]
     if num_ineq + num_eq != m:
@@ -177,6 +190,8 @@ def solve(params, Q, p, A0, zl, zu, num_ineq, num_eq, T, sigma, scaling=True, sc
         Upk16, wscale, Wx = packed.get_f16x3(params, h)
     else:
         Upk, Wx = packed.get(params, h)
+    if normed:
+        ln_w, ln_b = (params[k].detach().contiguous() for k in LN_NAMES)
     rho_p, alpha_p, b_h = (params[k].detach().contiguous() for k in ("rho", "alpha", "b_h"))
 
     f32 = dict(dtype=torch.float32, device=dev)
@@ -197,6 +212,9 @@ def solve(params, Q, p, A0, zl, zu, num_ineq, num_eq, T, sigma, scaling=True, sc
     xvs = [torch.zeros(B, N, **f32), torch.empty(B, N, **f32)]
     if f16:  # the fp32 H is written on the last iteration only (split planes per lane below)
         Hs = [torch.zeros(B, N, h, **f32)] * 2
+    elif normed:  # the cell reads the normalised state and writes over the one that it came from
+        Hs = [torch.zeros(B, N, h, **f32)] * 2
+        Hln = torch.empty(B, N, h, **f32)
     else:
         Hs = [torch.zeros(B, N, h, **f32), torch.empty(B, N, h, **f32)]
     C = torch.zeros(B, N, h, **f32)
@@ -249,13 +267,18 @@ def solve(params, Q, p, A0, zl, zu, num_ineq, num_eq, T, sigma, scaling=True, sc
         timer.stop(k)
         if t == 0 and L > 1:
             ln["kkt0"] = torch.cuda.current_stream(dev).record_event()
+        H_in = Hs[cur][sl]
+        if normed:
+            k = timer.start("k:layer_norm")
+            H_in = ops.layer_norm(H_in, ln_w, ln_b, LN_EPS, out=Hln[sl])
+            timer.stop(k)
         k = timer.start("k:lstm_cell")
         if f16:
             H16 = ln["H16"]
             ops.lstm_cell_f16x3(H16[cur], C[sl], xvs[cur][sl], g[sl], Upk16, wscale, Wx, Hn16=H16[nxt], Cn=C[sl],
                                 part=part, Hn=Hs[0][sl] if t == T - 1 else None)
         else:
-            ops.lstm_cell(Hs[cur][sl], C[sl], xvs[cur][sl], g[sl], Upk, Wx, Hn=Hs[nxt][sl], Cn=C[sl], part=part)
+            ops.lstm_cell(H_in, C[sl], xvs[cur][sl], g[sl], Upk, Wx, Hn=Hs[nxt][sl], Cn=C[sl], part=part)
         timer.stop(k)
         ops.admm_update(n, m, num_ineq, part, b_h, xvs[cur][sl], xs[cur][sl], ys[cur][sl], zs[cur][sl], zlv[sl],
                         zuv[sl], sc, out=(xvs[nxt][sl], xs[nxt][sl], ys[nxt][sl], zs[nxt][sl]))

@@ -58,6 +58,11 @@ def build_parser():
     add("--data_dir", type=str, default="./datasets")
     add("--micro_batch", type=int, default=0, help="instances per forward/backward pass (memory)")
     add("--max_minutes", type=float, default=0.0, help="train: stop after the epoch that exceeds this wall time")
+    add("--optimizer", type=str, choices=("adam", "adamw"), default="adam",
+        help="train: torch's Adam (the reference's) or the multi-tensor AdamW of iadmm/optim.py")
+    add("--state_bits", type=int, choices=(8, 32), default=32, help="train: bits of AdamW's moments")
+    add("--max_grad_norm", type=float, default=0.0, help="train: clip AdamW's gradients by their global norm (0: off)")
+    add("--layer_norm", action="store_true", help="a model that normalises the hidden state before the gates' product")
     add("--resume", type=str, default="", help="train: state file (model, Adam, epoch, EarlyStopping) written after "
                                                "every epoch and continued from when it exists")
     return p
@@ -75,6 +80,17 @@ def parse_args(argv=None):
         p.set_defaults(**{k: v for k, v in cfg.items() if k in known})
     args, _ = p.parse_known_args(argv)
     return args
+
+
+def make_optimizer(args, params):
+    """main.py:191's Adam, or iadmm.optim.AdamW with --optimizer adamw."""
+    if args.optimizer == "adam":
+        if args.state_bits != 32 or args.max_grad_norm:
+            raise SystemExit("--state_bits 8 and --max_grad_norm need --optimizer adamw")
+        return torch.optim.Adam(params, lr=args.lr, weight_decay=args.weight_decay)
+    from iadmm.optim import AdamW
+    return AdamW(params, lr=args.lr, weight_decay=args.weight_decay, state_bits=args.state_bits,
+                 max_norm=args.max_grad_norm or None, seed=args.seed)
 
 
 def split_ids(args):
@@ -133,7 +149,7 @@ def run_test(args):
     else:  # load first: the sizes of non-QP types come from the data
         allq = load_qp_instances(args, test_ids[:nb * tb], device)
     mi, me, n = args.num_ineq, args.num_eq, args.num_var
-    model = LSTM(mi + me, args.input_dim, args.hidden_dim, args.outer_T, device)
+    model = LSTM(mi + me, args.input_dim, args.hidden_dim, args.outer_T, device, layer_norm=args.layer_norm)
     ck = checkpoint_path(args, model.name())
     if os.path.exists(ck):
         model.load_state_dict(torch.load(ck, map_location=device, weights_only=True))
@@ -354,13 +370,13 @@ def run_train(args):
     dist = parallel.init("nccl", local) if world > 1 else None
     mi, me = args.num_ineq, args.num_eq
     torch.manual_seed(args.seed)
-    model = LSTM(mi + me, args.input_dim, args.hidden_dim, args.outer_T, device)
+    model = LSTM(mi + me, args.input_dim, args.hidden_dim, args.outer_T, device, layer_norm=args.layer_norm)
     save_path = os.path.join(args.save_dir, model.name(), "params", "QP_{}_{}_{}_{}_{}.pth".format(
         args.num_var, args.num_ineq, args.num_eq, args.outer_T, args.hidden_dim))  # main.py:88-92
     if rank == 0:
         os.makedirs(os.path.dirname(save_path), exist_ok=True)
     stopper = EarlyStopping(save_path, patience=args.patience)
-    optimizer = torch.optim.Adam(model.parameters(), lr=args.lr, weight_decay=args.weight_decay)
+    optimizer = make_optimizer(args, model.parameters())
     train_ids, val_ids, _ = split_ids(args)
     packed = solver.PackedWeights()
     history = []

@@ -8,7 +8,8 @@ runs three gfx950 kernels through libiadmm.so:
   iadmm_admm_update   xv / x / z / y updates                         (lstm.py:80-94)
 ``A_tild`` comes back as a lazy :class:`iadmm.kktop.KKTOperator` (``torch.bmm(A_tild, xv)``
 works; ``.dense()`` materialises K).  Outputs are fresh tensors (functional semantics): the
-caller may keep its inputs.  Under grad mode the call goes through
+caller may keep its inputs.  ``layer_norm=True`` (not in the reference) adds ``ln_w`` / ``ln_b`` [h] and
+normalises each coordinate's hidden state before the gates' product.  Under grad mode the call goes through
 :class:`iadmm.autograd.IterationFn`, whose backward is a set of HIP kernels (training).
 """
 import torch
@@ -17,8 +18,8 @@ import torch.nn as nn
 import iadmm_path  # noqa: F401
 from iadmm import ops
 from iadmm.kktop import KKTOperator
-from iadmm.autograd import IterationFn, window_grads_for
-from iadmm.solver import PARAM_NAMES, PackedWeights, param_dict
+from iadmm.autograd import IterationFn, layer_norm as layer_norm_fn, window_grads_for
+from iadmm.solver import LN_EPS, PARAM_NAMES, PackedWeights, param_dict
 
 _GATES = ("i", "f", "o", "u")
 
@@ -26,7 +27,7 @@ _GATES = ("i", "f", "o", "u")
 class LSTM(nn.Module):
     RHO_EQ_OVER_RHO_INEQ = 1e03  # fixed in the kernels (models/lstm.py:18)
 
-    def __init__(self, num_constr, input_dim, hidden_dim, length, device):
+    def __init__(self, num_constr, input_dim, hidden_dim, length, device, layer_norm=False):
         super().__init__()
         if input_dim != 2:
             raise ValueError("the I-ADMM-LSTM cell consumes [xv, K^T(K xv - b)]: input_dim must be 2")
@@ -51,6 +52,9 @@ class LSTM(nn.Module):
         self.b_h = zeros(1)
         self.rho = normal(length, 1)
         self.alpha = normal(length, 1)
+        if layer_norm:  # beyond the reference: H is normalised before the gates' product (same draws as without)
+            self.ln_w = nn.Parameter(torch.ones(hidden_dim, device=device, dtype=torch.float32))
+            self.ln_b = zeros(hidden_dim)
         self._packed = PackedWeights()
 
     def name(self):
@@ -81,7 +85,10 @@ class LSTM(nn.Module):
         g = ops.kkt_resgrad(Q, A0, pv, xv_, yv, zvv, xv2, float(sigma), scal, num_ineq,
                             btild=btild, rho_vec=rho_vec)
         Upk, Wx = self._packed.get(params, h)
-        Hn, Cn, part = ops.lstm_cell(c(H_t), c(C_t), xv2, g, Upk, Wx)
+        H_in = c(H_t)
+        if "ln_w" in params:
+            H_in = ops.layer_norm(H_in, c(params["ln_w"]), c(params["ln_b"]), LN_EPS)
+        Hn, Cn, part = ops.lstm_cell(H_in, c(C_t), xv2, g, Upk, Wx)
         xvo, xo, yo, zo = ops.admm_update(n, m, num_ineq, part, c(self.b_h), xv2, xv_, yv, zvv, zlv, zuv, scal)
         A_tild = KKTOperator(Q, A0, sigma, scal, num_ineq)
         return (xo.unsqueeze(-1), yo.unsqueeze(-1), zo.unsqueeze(-1), xvo.unsqueeze(-1), Hn, Cn,
@@ -97,6 +104,8 @@ class LSTM(nn.Module):
         Hc = H_t.float().contiguous()
         plist = [params[k] for k in PARAM_NAMES]
         acc, owner = window_grads_for(Hc, plist)  # the window's shared parameter-gradient sums (r06)
+        if "ln_w" in params:  # (the chain of iterations goes by H_t itself)
+            Hc = layer_norm_fn(Hc, params["ln_w"], params["ln_b"], LN_EPS)
         meta = (int(t), int(num_ineq), float(sigma), (Q, pv, A0, zlv, zuv), self._packed, acc, owner)
         xo, yo, zo, xvo, Hn, Cn, btild, rho_vec = IterationFn.apply(
             meta, flat(x, n), flat(y, m), flat(z, m), flat(xv, N), Hc, C_t.float().contiguous(), *plist)

@@ -94,3 +94,50 @@ def test_lists_are_checked():
     with pytest.raises(ValueError, match="contiguous"):
         ops.grad_norm([x.t()])
     ops.adamw_step([x], [None], [x], [x], 1)  # no gradient: nothing to do
+
+
+def test_optimizer_arguments():
+    from iadmm.optim import AdamW
+    p = [torch.nn.Parameter(torch.zeros(3))]
+    for kw in (dict(state_bits=16), dict(max_norm=0.0), dict(lr=-1.0), dict(lr=torch.tensor(1.0)), dict(betas=(1.0, 0.9)),
+               dict(eps=-1.0), dict(weight_decay=-1.0)):
+        with pytest.raises(ValueError):
+            AdamW(p, **kw)
+    with pytest.raises(TypeError):
+        AdamW([torch.nn.Parameter(torch.zeros(3, dtype=torch.float16))])
+    opt = AdamW(p)
+    assert opt.step() is None and not opt.state  # no gradient: nothing to do
+    p[0].grad = torch.ones(3)
+    with pytest.raises(ValueError, match="no CPU fallback"):
+        opt.step()
+
+
+def test_command_line_options():
+    import main
+    base = ["--lr", "0.1"]
+    args = main.parse_args(base)
+    assert args.optimizer == "adam" and not args.layer_norm
+    p = [torch.nn.Parameter(torch.zeros(3))]
+    assert type(main.make_optimizer(args, p)) is torch.optim.Adam
+    args = main.parse_args(base + ["--optimizer", "adamw", "--state_bits", "8", "--max_grad_norm", "2", "--weight_decay", "0.1"])
+    opt = main.make_optimizer(args, p)
+    assert (opt.state_bits, opt.max_norm, opt.defaults["lr"], opt.defaults["weight_decay"]) == (8, 2.0, 0.1, 0.1)
+    for extra in (["--state_bits", "8"], ["--max_grad_norm", "1"]):
+        with pytest.raises(SystemExit):
+            main.make_optimizer(main.parse_args(base + extra), p)
+
+
+def test_model_parameters_with_layer_norm():
+    """The reference's 16 parameters are drawn the same with and without; without, the model is the reference's."""
+    from models.lstm import LSTM
+    from iadmm import solver
+    models = []
+    for on in (False, True):
+        torch.manual_seed(1)
+        models.append(LSTM(4, 2, 8, 3, "cpu", layer_norm=on))
+    plain, normed = models
+    assert list(normed.state_dict()) == list(plain.state_dict()) + ["ln_w", "ln_b"]
+    assert all(torch.equal(v, normed.state_dict()[k]) for k, v in plain.state_dict().items())
+    assert list(solver.param_dict(plain)) == list(solver.PARAM_NAMES)
+    assert list(solver.param_dict(normed)) == list(solver.PARAM_NAMES) + list(solver.LN_NAMES)
+    assert list(solver.param_dict(dict(solver.param_dict(normed)))) == list(solver.PARAM_NAMES) + list(solver.LN_NAMES)
