@@ -91,6 +91,28 @@ template <bool FULL = false, typename T> IADMM_DEV void store_quad(T* p, const Q
   }
 }
 
+// The same for four codes, in one word (as members of their own they would be taken apart and put together again).
+template <bool FULL> IADMM_DEV uint32_t load_codes(const uint8_t* p, int64_t left) {
+  uint32_t r = 0;
+  if (FULL || left >= 4) {
+    __builtin_memcpy(&r, p, 4);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < left) r |= static_cast<uint32_t>(p[j]) << 8 * j;
+  }
+  return r;
+}
+template <bool FULL> IADMM_DEV void store_codes(uint8_t* p, uint32_t r, int64_t left) {
+  if (FULL || left >= 4) {
+    __builtin_memcpy(p, &r, 4);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < left) p[j] = static_cast<uint8_t>(r >> 8 * j);
+  }
+}
+
 IADMM_DEV float bits_f(uint32_t b) { return __uint_as_float(b); }
 IADMM_DEV bool is_finite(float x) { return fabsf(x) < __builtin_inff(); }
 
@@ -118,20 +140,21 @@ IADMM_DEV int block_exponent(uint32_t top, int shift, int low, int high) {
   const int e = static_cast<int>((top + 0x200000u) >> 23) - 127 - shift;
   return e < low ? low : (e > high ? high : e);
 }
-// The largest of the wave's values, as a scalar: six maxima whose second operand comes from another lane (within
-// rows of 16, then across them) instead of twelve instructions through LDS.
+// The largest of the wave's values, as scalars: six maxima whose second operand comes from another lane (within rows
+// of 16, then across them) instead of twelve instructions through LDS; two at a time, each in the other's wait states.
 template <int CTRL> IADMM_DEV uint32_t umax_from(uint32_t v) {
   const uint32_t w = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, 0xF, 0xF, false));
   return w > v ? w : v;
 }
-IADMM_DEV uint32_t wave_umax(uint32_t v) {
-  v = umax_from<0x111>(v);  // row_shr 1, 2, 4, 8: lane 15 of each row has its row's
-  v = umax_from<0x112>(v);
-  v = umax_from<0x114>(v);
-  v = umax_from<0x118>(v);
-  v = umax_from<0x142>(v);  // row_bcast 15, 31: lane 63 has the wave's
-  v = umax_from<0x143>(v);
-  return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), 63));
+IADMM_DEV void wave_umax(uint32_t& a, uint32_t& b) {
+  a = umax_from<0x111>(a), b = umax_from<0x111>(b);  // row_shr 1, 2, 4, 8: lane 15 of each row has its row's
+  a = umax_from<0x112>(a), b = umax_from<0x112>(b);
+  a = umax_from<0x114>(a), b = umax_from<0x114>(b);
+  a = umax_from<0x118>(a), b = umax_from<0x118>(b);
+  a = umax_from<0x142>(a), b = umax_from<0x142>(b);  // row_bcast 15, 31: lane 63 has the wave's
+  a = umax_from<0x143>(a), b = umax_from<0x143>(b);
+  a = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(a), 63));
+  b = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(b), 63));
 }
 
 // Four codes at once, as the dword that they lie in.  The scales are products here, so the exponents have to
@@ -144,20 +167,20 @@ IADMM_DEV bool ordinary_codes(uint32_t m, uint32_t v) {  // no NaN (m & 127 = 12
   return ((a | b) & 0x80808080u) == 0u;
 }
 template <int J> IADMM_DEV float decode_m_of(uint32_t q, float scale) {
-  const uint32_t mag = J < 3 ? q << (20 - 8 * J) : q >> 4, sign = q << (24 - 8 * J);
-  return bits_f((__float_as_uint(bits_f(mag & 0x07F00000u) * scale) & 0x7FFFFFFFu) | (sign & 0x80000000u));
+  const int t = static_cast<int>(q << (24 - 8 * J));  // the sign in place; shifted on, it is above the magnitude
+  return bits_f(static_cast<uint32_t>(t >> 4) & 0x87F00000u) * scale;
 }
 template <int J> IADMM_DEV float decode_v_of(uint32_t q, float scale) {
-  return bits_f((J < 3 ? q << (20 - 8 * J) : q >> 4) & 0x0FF00000u) * scale;
+  return bits_f((q >> 8 * J & 255u) << 20) * scale;
 }
-// The code in the top byte.
+// The code in the top byte (the blocks' exponents keep it below NaN's and infinity's).
 IADMM_DEV uint32_t encode_m_top(float m, float scale, uint32_t bits) {
   const uint32_t a = (__float_as_uint(fabsf(m) * scale) + (bits >> 20 << 8)) << 4;
-  return (a & 0x7FFFFFFFu) | (__float_as_uint(m) & 0x80000000u);
+  return (__float_as_uint(m) & 0x80000000u) | a;
 }
 IADMM_DEV uint32_t encode_v_top(float v, float scale, uint32_t bits) {
-  const uint32_t a = __float_as_uint(v * scale) + (bits & 0xFFFFFu), b = __float_as_uint(v), one = (b < 1u ? b : 1u) << 20;
-  return (a > one ? a : one) << 4;
+  const uint32_t a = __float_as_uint(v * scale) + (bits & 0xFFFFFu), one = 1u << 20;
+  return (v > 0.0f && a < one ? one : a) << 4;
 }
 IADMM_DEV uint32_t top_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   const uint32_t lo = __builtin_amdgcn_perm(b, a, 0x00000703u), hi = __builtin_amdgcn_perm(d, c, 0x07030000u);
@@ -180,55 +203,74 @@ template <typename L> IADMM_DEV int find_tensor(const L& a, uint32_t block) {
 struct AdamScalars {
   float step_size, ibc2, decay, clip;
   uint32_t key;
-  bool clipped;
 };
 
-// QUADS x 256 elements per wave, a workgroup's four waves beside each other.
+// The new parameters of four elements; `bits` are 0 for fp32.  SAFE: NaN keeps its bits (random ones added to a payload
+// of ones would carry into the sign; where the moments are finite, a NaN is a bf16 parameter's own, with lower bits 0).
+template <typename P, bool SAFE> IADMM_DEV Quad<P> new_params(const float (&np)[4], const uint32_t (&bits)[4]) {
+  Quad<P> q;
+  if constexpr (sizeof(P) == 2) {
+    uint32_t b[4], w[2];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      b[j] = __float_as_uint(np[j]) + (bits[j] >> 16);
+      if (SAFE) b[j] = np[j] != np[j] ? 0x7FC00000u : b[j];
+    }
+    w[0] = __builtin_amdgcn_perm(b[1], b[0], 0x07060302u);
+    w[1] = __builtin_amdgcn_perm(b[3], b[2], 0x07060302u);
+    __builtin_memcpy(&q, w, 8);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) q.v[j] = np[j];
+  }
+  return q;
+}
+
+// QUADS x 256 elements per wave.
 template <typename P, typename G, bool EIGHT, int QUADS, bool FULL>
 IADMM_DEV void adam_wave(const AdamLaunch& a, const AdamTensor& t, const AdamScalars& s, int64_t at) {
-  using S = typename std::conditional<EIGHT, uint8_t, float>::type;
   const int lane = threadIdx.x % kWave;
   P* p = static_cast<P*>(t.p);
   const G* g = static_cast<const G*>(t.g);
-  S *m = static_cast<S*>(t.m), *v = static_cast<S*>(t.v);
-  int8_t* e = static_cast<int8_t*>(t.e);
+  float *m = static_cast<float*>(t.m), *v = static_cast<float*>(t.v);
+  uint8_t *m8 = static_cast<uint8_t*>(t.m), *v8 = static_cast<uint8_t*>(t.v);
+  int8_t* e = static_cast<int8_t*>(t.e) + at / kBlock8 * 2;
   Quad<P> qp[QUADS];
   Quad<G> qg[QUADS];
-  Quad<S> qm[QUADS], qv[QUADS];
-  int em[QUADS], ev[QUADS];
+  Quad<float> qm[QUADS], qv[QUADS];
+  uint32_t cm[QUADS], cv[QUADS];
+  int8_t old[2 * QUADS], now[2 * QUADS];
 #pragma unroll
   for (int u = 0; u < QUADS; ++u) {
     const int64_t i = at + u * 256 + lane * 4, left = t.n - i;
     qp[u] = load_quad<FULL>(p + i, left);
     qg[u] = load_quad<FULL>(g + i, left);
-    qm[u] = load_quad<FULL>(m + i, left);
-    qv[u] = load_quad<FULL>(v + i, left);
-    em[u] = ev[u] = 0;
-    if (EIGHT && (FULL || at + u * 256 < t.n)) {
-      em[u] = e[(at + u * 256) / kBlock8 * 2];
-      ev[u] = e[(at + u * 256) / kBlock8 * 2 + 1];
+    if constexpr (EIGHT) {
+      cm[u] = load_codes<FULL>(m8 + i, left);
+      cv[u] = load_codes<FULL>(v8 + i, left);
+    } else {
+      qm[u] = load_quad<FULL>(m + i, left);
+      qv[u] = load_quad<FULL>(v + i, left);
     }
   }
+  if constexpr (EIGHT) __builtin_memcpy(old, e, 2 * QUADS);  // (every quad here has elements)
 #pragma unroll
   for (int u = 0; u < QUADS; ++u) {
-    if (!FULL && at + u * 256 >= t.n) break;  // (the whole wave)
     const int64_t i = at + u * 256 + lane * 4, left = t.n - i;
     float fm[4], fv[4], np[4];
     uint32_t bits[4] = {0, 0, 0, 0};
     const uint32_t place = static_cast<uint32_t>(i) + static_cast<uint32_t>(i >> 32) * 0x9E3779B9u;  // (i % 4 = 0: no carry)
     if constexpr (EIGHT) {
-      uint32_t cm, cv;
-      __builtin_memcpy(&cm, &qm[u], 4);
-      __builtin_memcpy(&cv, &qv[u], 4);
-      if (em[u] <= kFastM && ev[u] <= kFastV && __all(ordinary_codes(cm, cv))) {
-        const float sm = pow2(em[u] + 120), sv = pow2(ev[u] + 96);
-        fm[0] = decode_m_of<0>(cm, sm), fm[1] = decode_m_of<1>(cm, sm);
-        fm[2] = decode_m_of<2>(cm, sm), fm[3] = decode_m_of<3>(cm, sm);
-        fv[0] = decode_v_of<0>(cv, sv), fv[1] = decode_v_of<1>(cv, sv);
-        fv[2] = decode_v_of<2>(cv, sv), fv[3] = decode_v_of<3>(cv, sv);
+      const int em = __builtin_amdgcn_readfirstlane(old[2 * u]), ev = __builtin_amdgcn_readfirstlane(old[2 * u + 1]);
+      if (em <= kFastM && ev <= kFastV && __all(ordinary_codes(cm[u], cv[u]))) {
+        const float sm = pow2(em + 120), sv = pow2(ev + 96);
+        fm[0] = decode_m_of<0>(cm[u], sm), fm[1] = decode_m_of<1>(cm[u], sm);
+        fm[2] = decode_m_of<2>(cm[u], sm), fm[3] = decode_m_of<3>(cm[u], sm);
+        fv[0] = decode_v_of<0>(cv[u], sv), fv[1] = decode_v_of<1>(cv[u], sv);
+        fv[2] = decode_v_of<2>(cv[u], sv), fv[3] = decode_v_of<3>(cv[u], sv);
       } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) fm[j] = decode_m(cm >> 8 * j & 255u, em[u]), fv[j] = decode_v(cv >> 8 * j & 255u, ev[u]);
+        for (int j = 0; j < 4; ++j) fm[j] = decode_m(cm[u] >> 8 * j & 255u, em), fv[j] = decode_v(cv[u] >> 8 * j & 255u, ev);
       }
     } else {
 #pragma unroll
@@ -236,36 +278,27 @@ IADMM_DEV void adam_wave(const AdamLaunch& a, const AdamTensor& t, const AdamSca
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      float gr = static_cast<float>(qg[u].v[j]);
-      if (s.clipped) gr = gr * s.clip;
+      const float gr = static_cast<float>(qg[u].v[j]) * s.clip;
       fm[j] = a.b1 * fm[j] + a.ob1 * gr;
       fv[j] = a.b2 * fv[j] + a.ob2 * (gr * gr);
-      const float old = static_cast<float>(qp[u].v[j]) * s.decay;
+      const float kept = static_cast<float>(qp[u].v[j]) * s.decay;
       if constexpr (EIGHT) {
         // the hardware's root and reciprocal, 1 ulp each: with 8-bit moments the arithmetic takes as long as the
         // memory, and their correctly rounded forms are a third of it
         const float d = __builtin_amdgcn_sqrtf(fv[j]) * s.ibc2 + a.eps;
-        np[j] = old - s.step_size * (fm[j] * __builtin_amdgcn_rcpf(d));
+        np[j] = kept - s.step_size * (fm[j] * __builtin_amdgcn_rcpf(d));
       } else {
-        np[j] = old - s.step_size * (fm[j] / (sqrtf(fv[j]) * s.ibc2 + a.eps));
+        np[j] = kept - s.step_size * (fm[j] / (sqrtf(fv[j]) * s.ibc2 + a.eps));
       }
-      if constexpr (EIGHT || sizeof(P) == 2) {
-        bits[j] = mix32((place + j) ^ s.key);
-      }
+      if constexpr (EIGHT || sizeof(P) == 2) bits[j] = mix32((place + j) ^ s.key);
     }
-    if constexpr (sizeof(P) == 2) {
+    if constexpr (!EIGHT) {
+      store_quad<FULL>(p + i, new_params<P, true>(np, bits), left);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t b = (__float_as_uint(np[j]) + (bits[j] >> 16)) >> 16;
-        const uint16_t h = static_cast<uint16_t>(np[j] != np[j] ? 0x7FC0u : b);
-        __builtin_memcpy(&qp[u].v[j], &h, 2);
-      }
+      for (int j = 0; j < 4; ++j) qm[u].v[j] = fm[j], qv[u].v[j] = fv[j];
+      store_quad<FULL>(m + i, qm[u], left);
+      store_quad<FULL>(v + i, qv[u], left);
     } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) qp[u].v[j] = np[j];
-    }
-    store_quad<FULL>(p + i, qp[u], left);
-    if constexpr (EIGHT) {
       uint32_t tm = 0, tv = 0;  // (elements behind the end are 0; v is never negative)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -273,18 +306,20 @@ IADMM_DEV void adam_wave(const AdamLaunch& a, const AdamTensor& t, const AdamSca
         tm = bm > tm ? bm : tm;
         tv = bv > tv ? bv : tv;
       }
-      tm = wave_umax(tm);
-      tv = wave_umax(tv);
+      wave_umax(tm, tv);
       int ne = block_exponent(tm, 8, -117, 120), nv = block_exponent(tv, 0, -93, 127);
       if (tm < 0x7F800000u && tv < 0x7F800000u && ne <= kFastM && nv <= kFastV) {
+        store_quad<FULL>(p + i, new_params<P, false>(np, bits), left);
         const float sm = pow2(-ne - 120), sv = pow2(-nv - 96);
-        uint32_t cm[4], cv[4];
+        uint32_t tops[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) cm[j] = encode_m_top(fm[j], sm, bits[j]), cv[j] = encode_v_top(fv[j], sv, bits[j]);
-        const uint32_t pm = top_bytes(cm[0], cm[1], cm[2], cm[3]), pv = top_bytes(cv[0], cv[1], cv[2], cv[3]);
-        __builtin_memcpy(&qm[u], &pm, 4);
-        __builtin_memcpy(&qv[u], &pv, 4);
+        for (int j = 0; j < 4; ++j) tops[j] = encode_m_top(fm[j], sm, bits[j]);
+        cm[u] = top_bytes(tops[0], tops[1], tops[2], tops[3]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) tops[j] = encode_v_top(fv[j], sv, bits[j]);
+        cv[u] = top_bytes(tops[0], tops[1], tops[2], tops[3]);
       } else {  // the exponents are the finite values'
+        store_quad<FULL>(p + i, new_params<P, true>(np, bits), left);
         tm = tv = 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -293,25 +328,24 @@ IADMM_DEV void adam_wave(const AdamLaunch& a, const AdamTensor& t, const AdamSca
           tm = bm > tm ? bm : tm;
           tv = bv > tv ? bv : tv;
         }
-        ne = block_exponent(wave_umax(tm), 8, -117, 120);
-        nv = block_exponent(wave_umax(tv), 0, -93, 127);
+        wave_umax(tm, tv);
+        ne = block_exponent(tm, 8, -117, 120);
+        nv = block_exponent(tv, 0, -93, 127);
+        cm[u] = cv[u] = 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          qm[u].v[j] = static_cast<uint8_t>(encode_m(fm[j], ne, bits[j]));
-          qv[u].v[j] = static_cast<uint8_t>(encode_v(fv[j], nv, bits[j]));
+          cm[u] |= encode_m(fm[j], ne, bits[j]) << 8 * j;
+          cv[u] |= encode_v(fv[j], nv, bits[j]) << 8 * j;
         }
       }
-      if (lane == 0) {
-        e[(at + u * 256) / kBlock8 * 2] = static_cast<int8_t>(ne);
-        e[(at + u * 256) / kBlock8 * 2 + 1] = static_cast<int8_t>(nv);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) qm[u].v[j] = fm[j], qv[u].v[j] = fv[j];
+      now[2 * u] = static_cast<int8_t>(ne);
+      now[2 * u + 1] = static_cast<int8_t>(nv);
+      store_codes<FULL>(m8 + i, cm[u], left);
+      store_codes<FULL>(v8 + i, cv[u], left);
     }
-    store_quad<FULL>(m + i, qm[u], left);
-    store_quad<FULL>(v + i, qv[u], left);
   }
+  if constexpr (EIGHT)
+    if (lane == 0) __builtin_memcpy(e, now, 2 * QUADS);
 }
 
 template <typename P, typename G, bool EIGHT, int QUADS>
@@ -329,7 +363,7 @@ IADMM_DEV void adam_chunk(const AdamLaunch& a, const AdamTensor& t, const AdamSc
 template <bool EIGHT, int QUADS> __global__ void __launch_bounds__(256) adam_kernel(const AdamLaunch a) {
   const int k = find_tensor(a, blockIdx.x);
   const AdamTensor& t = a.t[k];
-  AdamScalars s{t.step_size, t.ibc2, a.decay, 1.0f, t.key, a.norm != nullptr};
+  AdamScalars s{t.step_size, t.ibc2, a.decay, 1.0f, t.key};
   if (a.table) {
     const float4 f = a.table[k];
     s.step_size = f.x;
