@@ -456,20 +456,19 @@ struct NormLaunch {
   uint32_t chunks;
   int count;
 };
-constexpr int kNormChunk = 8192;  // elements
 
 // Squares in 64 bits: they neither overflow (fp32's do from 1.8e19 on) nor lose small tensors beside large ones;
 // the conversion and the product cost a third of the time that the bytes take.
-template <typename T, bool FULL> IADMM_DEV double square_sum_of(const T* g, int64_t at, int64_t n) {
-  Quad<T> q[8];
+template <typename T, int QUADS, bool FULL> IADMM_DEV double square_sum_of(const T* g, int64_t at, int64_t n) {
+  Quad<T> q[QUADS];
 #pragma unroll
-  for (int u = 0; u < 8; ++u) {
+  for (int u = 0; u < QUADS; ++u) {
     const int64_t i = at + u * 1024 + threadIdx.x * 4;
     q[u] = load_quad<FULL>(g + i, n - i);
   }
   double s = 0.0;
 #pragma unroll
-  for (int u = 0; u < 8; ++u)
+  for (int u = 0; u < QUADS; ++u)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const double d = static_cast<double>(static_cast<float>(q[u].v[j]));
@@ -477,9 +476,9 @@ template <typename T, bool FULL> IADMM_DEV double square_sum_of(const T* g, int6
     }
   return s;
 }
-template <typename T> IADMM_DEV double square_sum(const void* g, int64_t at, int64_t n) {
+template <typename T, int QUADS> IADMM_DEV double square_sum(const void* g, int64_t at, int64_t n) {
   const T* p = static_cast<const T*>(g);
-  return at + kNormChunk <= n ? square_sum_of<T, true>(p, at, n) : square_sum_of<T, false>(p, at, n);
+  return at + QUADS * 1024 <= n ? square_sum_of<T, QUADS, true>(p, at, n) : square_sum_of<T, QUADS, false>(p, at, n);
 }
 
 IADMM_DEV double block_sum_f64(double s, double* red) {
@@ -492,7 +491,7 @@ IADMM_DEV double block_sum_f64(double s, double* red) {
   return s;
 }
 
-__global__ void __launch_bounds__(256) norm_kernel(const NormLaunch a) {
+template <int QUADS> __global__ void __launch_bounds__(256) norm_kernel(const NormLaunch a) {
   __shared__ double red[4];
   // a run of neighbouring chunks, so that the tensor is looked for once
   uint32_t c = static_cast<uint32_t>(static_cast<uint64_t>(a.chunks) * blockIdx.x / gridDim.x);
@@ -502,8 +501,8 @@ __global__ void __launch_bounds__(256) norm_kernel(const NormLaunch a) {
   for (; c < end; ++c) {
     while (k + 1 < a.count && a.t[k + 1].first <= c) ++k;
     const NormTensor& t = a.t[k];
-    const int64_t at = static_cast<int64_t>(c - t.first) * kNormChunk;
-    s += t.half ? square_sum<__bf16>(t.g, at, t.n) : square_sum<float>(t.g, at, t.n);
+    const int64_t at = static_cast<int64_t>(c - t.first) * (QUADS * 1024);
+    s += t.half ? square_sum<__bf16, QUADS>(t.g, at, t.n) : square_sum<float, QUADS>(t.g, at, t.n);
   }
   s = block_sum_f64(s, red);
   if (threadIdx.x == 0) a.part[blockIdx.x] = s;
@@ -517,6 +516,25 @@ __global__ void __launch_bounds__(1024) norm_end_kernel(const double* part, int 
   if (threadIdx.x == 0) *norm = static_cast<float>(sqrt(s));
 }
 
+// Workgroups take 2048 elements at a time up to this many in all, 8192 above: 168 000 of them 7.1 us against 7.7 (with the
+// last sum's launch), 2.6 M 8.2 against 8.0.
+constexpr int64_t kNormSmall = int64_t{1} << 19;
+template <int QUADS> static int launch_norm(NormLaunch& a, hipStream_t st) {  // the workgroups, or an error
+  uint64_t chunks = 0;
+  for (int k = 0; k < a.count; ++k) {
+    a.t[k].first = static_cast<uint32_t>(chunks);
+    chunks += (static_cast<uint64_t>(a.t[k].n) + QUADS * 1024 - 1) / (QUADS * 1024);
+    if (chunks > 0x7FFFFFFFu) return IADMM_E_SIZE;
+  }
+  a.chunks = static_cast<uint32_t>(chunks);
+  const int blocks = chunks < kNormBlocks ? static_cast<int>(chunks) : kNormBlocks;
+  hipLaunchKernelGGL(norm_kernel<QUADS>, dim3(blocks), dim3(256), 0, st, a);
+  return blocks;
+}
+
+// Workgroups of 1024 elements up to this many in all, of 4096 above: 168 000 of them 7.9 us against 8.9 (with the
+// counting launch), 2.6 M 17.9 against 16.6.
+constexpr int64_t kAdamSmall = int64_t{1} << 19;
 template <bool EIGHT, int QUADS> static int launch_adam(AdamLaunch& a, hipStream_t st) {
   uint64_t blocks = 0;
   for (int k = 0; k < a.count; ++k) {
@@ -552,22 +570,20 @@ extern "C" int iadmm_grad_norm(int64_t count, const iadmm_grad_tensor* grads, fl
   int parts = 0;
   NormLaunch a;
   a.count = 0;
-  uint64_t chunks = 0;
+  int64_t total = 0;
   for (int64_t i = 0; i < count; ++i) {
     if (grads[i].n > 0) {
-      a.t[a.count++] = NormTensor{grads[i].g, grads[i].n, static_cast<uint32_t>(chunks), grads[i].dtype == IADMM_BF16};
-      chunks += (static_cast<uint64_t>(grads[i].n) + kNormChunk - 1) / kNormChunk;
-      if (chunks > 0x7FFFFFFFu) return IADMM_E_SIZE;
+      a.t[a.count++] = NormTensor{grads[i].g, grads[i].n, 0u, grads[i].dtype == IADMM_BF16};
+      total += grads[i].n;
     }
     if (a.count > 0 && (a.count == kNormPer || i == count - 1)) {
-      const int blocks = chunks < kNormBlocks ? static_cast<int>(chunks) : kNormBlocks;
-      a.chunks = static_cast<uint32_t>(chunks);
       a.part = part + parts;
-      hipLaunchKernelGGL(norm_kernel, dim3(blocks), dim3(256), 0, st, a);
+      const int blocks = total <= kNormSmall ? launch_norm<2>(a, st) : launch_norm<8>(a, st);
+      if (blocks < 0) return blocks;
       IADMM_CHECK_LAUNCH();
       parts += blocks;
       a.count = 0;
-      chunks = 0;
+      total = 0;
     }
   }
   hipLaunchKernelGGL(norm_end_kernel, dim3(1), dim3(1024), 0, st, part, parts, norm);
@@ -629,7 +645,9 @@ extern "C" int iadmm_adamw_step(int64_t count, const iadmm_adamw_tensor* tensors
       IADMM_CHECK_LAUNCH();
     }
     if (total == 0) continue;
-    const int rc = eight ? launch_adam<true, 4>(a, st) : launch_adam<false, 4>(a, st);
+    const bool small = total <= kAdamSmall;
+    const int rc = eight ? (small ? launch_adam<true, 1>(a, st) : launch_adam<true, 4>(a, st))
+                         : (small ? launch_adam<false, 1>(a, st) : launch_adam<false, 4>(a, st));
     if (rc) return rc;
   }
   return IADMM_OK;

@@ -96,12 +96,15 @@ template <typename T> IADMM_DEV void store_pack(T* p, const Pack<T>& r, int64_t 
   }
 }
 
-// V weights from column c, of type T or fp32; `none` where there are none.  WHOLE: all within the row.
-template <typename T, bool WHOLE = false> IADMM_DEV void load_weights(const void* w, bool f32, int64_t c, int64_t cols,
-                                                                      float none, float* out) {
+// V weights from column c, of type T or fp32; `none` where there are none.  WHOLE: all within the row.  KIND: which
+// of these it is, where the caller has asked already (outside its loop, whose loads a branch would keep apart).
+enum { kAnyKind, kFloats, kSame };
+template <typename T, bool WHOLE = false, int KIND = kAnyKind>
+IADMM_DEV void load_weights(const void* w, bool f32, int64_t c, int64_t cols, float none, float* out) {
   constexpr int V = Pack<T>::n;
   const int64_t n = WHOLE ? V : cols - c;
-  if (!w) {
+  f32 = KIND == kFloats || (KIND == kAnyKind && f32);
+  if (KIND == kAnyKind && !w) {
 #pragma unroll
     for (int j = 0; j < V; ++j) out[j] = none;
   } else if (sizeof(T) == 4 || f32) {
@@ -197,19 +200,23 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) ln_fwd_kernel(LnFwd a) 
   const float r = 1.0f / sqrtf(s[0] * inv + a.eps);
   if (!on) return;
   T* y = static_cast<T*>(a.y) + row * a.cols;
+  auto finish = [&](auto kind) {
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int64_t c = static_cast<int64_t>(i * TPR + lane) * V;
-    if (c >= a.cols) continue;
-    const int64_t at = SHORT ? c : place<T>(c, a.cols).at;
-    float w[V], b[V];
-    load_weights<T, !SHORT>(a.w, a.w32, at, a.cols, 1.0f, w);
-    load_weights<T, !SHORT>(a.b, a.w32, at, a.cols, 0.0f, b);
+    for (int i = 0; i < NV; ++i) {
+      const int64_t c = static_cast<int64_t>(i * TPR + lane) * V;
+      const int64_t at = SHORT ? c : place<T>(c, a.cols).at;
+      float w[V], b[V];
+      load_weights<T, !SHORT, kind()>(a.w, a.w32, at, a.cols, 1.0f, w);
+      load_weights<T, !SHORT, kind()>(a.b, a.w32, at, a.cols, 0.0f, b);
 #pragma unroll
-    for (int j = 0; j < V; ++j) w[j] = fmaf((get(p[i], j) - mu) * r, w[j], b[j]);
-    set(p[i], w);
-    store_pack(y + at, p[i], SHORT ? a.cols - at : V);
-  }
+      for (int j = 0; j < V; ++j) w[j] = fmaf((get(p[i], j) - mu) * r, w[j], b[j]);
+      set(p[i], w);
+      if (c < a.cols) store_pack(y + at, p[i], SHORT ? a.cols - at : V);
+    }
+  };
+  if (!a.w || !a.b || SHORT) finish(std::integral_constant<int, kAnyKind>());
+  else if (sizeof(T) == 4 || a.w32) finish(std::integral_constant<int, kFloats>());
+  else finish(std::integral_constant<int, kSame>());
   if (lane == 0 && a.mean) a.mean[row] = mu;
   if (lane == 0 && a.rstd) a.rstd[row] = r;
 }
@@ -493,7 +500,10 @@ static int row_threads_bwd(int64_t cols, int vec) {
   if (cols <= 16 * 16) return vec == 8 || cols <= 16 * 8 ? 16 : 64;
   return cols <= 64 * 32 ? 64 : cols <= 256 * 16 ? 256 : 1024;
 }
-static int bwd_block(int64_t cols, int tpr) { return tpr == 64 && cols > 64 * 16 ? 512 : 1024; }
+static int bwd_block(int64_t cols, int tpr) { return tpr == 256 || (tpr == 64 && cols > 64 * 16) ? 512 : 1024; }
+// Workgroups, and so slabs: one per CU; two where they are of 512 threads that meet at barriers, so that one loads
+// while the other waits.
+static int64_t bwd_most(int tpr) { return tpr == 256 ? 2 * kCUs : kCUs; }
 
 static int64_t bwd_slabs(int64_t rows, int64_t cols, int vec) {
   if (rows <= 0) return 0;
@@ -505,7 +515,7 @@ static int64_t bwd_slabs(int64_t rows, int64_t cols, int vec) {
   const int tpr = row_threads_bwd(cols, vec);
   const int64_t per = bwd_block(cols, tpr) / tpr;
   const int64_t need = (rows + per - 1) / per;
-  return need < kCUs ? need : kCUs;
+  return need < bwd_most(tpr) ? need : bwd_most(tpr);
 }
 
 template <typename T, int TPR, int NV, bool SHORT = false> static void launch_fwd(const LnFwd& a, hipStream_t st) {
@@ -570,7 +580,7 @@ template <typename T> static int bwd(const LnBwd& a, int64_t slabs, hipStream_t 
       if (nv <= 4) return launch_bwd<T, 64, 4>(a, slabs, st);
     return launch_bwd<T, 64, 2 * M, 512>(a, slabs, st);
   }
-  if (tpr == 256) return launch_bwd<T, 256, M>(a, slabs, st);
+  if (tpr == 256) return launch_bwd<T, 256, M, 512>(a, slabs, st);
   return nv <= M / 2 ? launch_bwd<T, 1024, M / 2>(a, slabs, st) : launch_bwd<T, 1024, M>(a, slabs, st);
 }
 

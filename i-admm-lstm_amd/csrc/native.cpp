@@ -81,6 +81,17 @@ void check_row_vector(const Tensor& w, const Tensor& x, int64_t cols, const char
 const void* address(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 void* address_of(Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
 
+// Whether two tensors' memory has a byte in common.
+bool overlap(const Tensor& a, const Tensor& b) {
+  if (!a.defined() || !b.defined() || !a.numel() || !b.numel()) return false;
+  auto end = [](const Tensor& t) {
+    int64_t last = 0;
+    for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+    return static_cast<const char*>(t.const_data_ptr()) + (last + 1) * static_cast<int64_t>(t.element_size());
+  };
+  return static_cast<const char*>(a.const_data_ptr()) < end(b) && static_cast<const char*>(b.const_data_ptr()) < end(a);
+}
+
 Tensor ln_forward(const Tensor& x, const Tensor& w, const Tensor& b, double eps, Tensor out, Tensor* mean, Tensor* rstd) {
   on_device(x, "x");
   const int t = type_code(x.scalar_type());
@@ -95,6 +106,9 @@ Tensor ln_forward(const Tensor& x, const Tensor& w, const Tensor& b, double eps,
     on_device(out, "out", &x);
     TORCH_CHECK_VALUE(out.sizes() == x.sizes() && out.scalar_type() == x.scalar_type() && out.is_contiguous(),
                       "out must be contiguous ", x.sizes(), " ", x.scalar_type());
+    TORCH_CHECK_VALUE(!overlap(out, w) && !overlap(out, b) &&
+                      (!overlap(out, x) || (x.is_contiguous() && out.const_data_ptr() == x.const_data_ptr())),
+                      "out may be x itself, and may not overlap it, weight or bias otherwise");
   } else {
     out = at::empty(x.sizes(), x.options());
   }
@@ -341,7 +355,7 @@ PyObject* py_adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
   want(n, 14);
   const Fast params(a[0], "params must be a list"), grads(a[1], "grads must be a list"),
       avgs(a[2], "exp_avgs must be a list"), sqs(a[3], "exp_avg_sqs must be a list");
-  const bool eight = a[4] != Py_None, counted = THPVariable_Check(a[5]), numbers = !counted && !PyLong_Check(a[5]);
+  const bool eight = a[4] != Py_None, counted = THPVariable_Check(a[5]), numbers = !counted && !PyIndex_Check(a[5]);
   const Fast exps(eight ? a[4] : a[0], "exponents must be a list");
   const Fast steps(numbers ? a[5] : a[0], "step must be a number, a list of numbers or a tensor");
   const int count = params.size();

@@ -500,6 +500,16 @@ def test_refusals_change_nothing():
     assert all(torch.equal(a, b) for a, b in zip(keep, P + M + V))
 
 
+def test_numbers_of_numpy():
+    from iadmm import ops
+    A, C = tensors([100]), tensors([100])
+    ops.adamw_step(*A[:4], np.int64(3), lr=np.float64(1e-3))
+    ops.adamw_step(*C[:4], [np.int32(3)], lr=1e-3)
+    assert torch.equal(A[0][0], C[0][0])
+    with pytest.raises((TypeError, ValueError)):
+        ops.adamw_step(*A[:4], 3.5)
+
+
 def test_a_step_is_seen_by_the_version():
     """solver.PackedWeights goes by a parameter's version: a step has to raise it."""
     from iadmm import ops

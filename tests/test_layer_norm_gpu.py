@@ -166,7 +166,10 @@ def test_no_rows_and_refusals():
     bad = [dict(x=x.double()), dict(x=x.t()), dict(x=x[:, :0]), dict(x=torch.zeros((), device="cuda")), dict(x=x, weight=w[:7]),
            dict(x=x, weight=w.half()), dict(x=x, weight=w.cpu()), dict(x=x.half(), weight=w, bias=w.half()),
            dict(x=x, eps=-1.0), dict(x=x, eps=float("nan")), dict(x=x, out=x.half()), dict(x=x, out=x[:2]),
-           dict(x=x[:1].expand(4, 8)), dict(x=x.cpu())]
+           dict(x=x[:1].expand(4, 8)), dict(x=x.cpu()), dict(x=x[:3], out=x[1:]), dict(x=x[:1], weight=w, out=w.view(1, 8)),
+           dict(x=torch.zeros(4, 9, device="cuda")[:, :8], out=torch.zeros(4, 9, device="cuda").view(-1)[:32].view(8, 4))]
+    wide = torch.zeros(4, 9, device="cuda")
+    bad.append(dict(x=wide[:, :8], out=wide.view(-1)[:32].view(4, 8)))
     for kw in bad:
         with pytest.raises((TypeError, ValueError, _abi.IadmmError)):
             ops.layer_norm(**kw)
