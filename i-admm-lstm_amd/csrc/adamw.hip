@@ -54,13 +54,13 @@ struct AdamLaunch {
 
 // 32 well-mixed bits of 32: two odd multipliers between shifts, chosen by search for the least bias of any
 // output bit's flip under any input bit's (0.4 % at most over 200 000 inputs).
-__host__ __device__ inline uint32_t mix32(uint32_t x) {
-  x ^= x >> 16;
+__host__ __device__ inline uint32_t mix32_rest(uint32_t x) {
   x *= 0xDEFBD895u;
   x ^= x >> 15;
   x *= 0x066B4493u;
   return x ^ (x >> 16);
 }
+__host__ __device__ inline uint32_t mix32(uint32_t x) { return mix32_rest(x ^ x >> 16); }
 __host__ __device__ inline uint32_t step_key(uint64_t seed, uint64_t step, int slot) {
   uint32_t k = mix32(static_cast<uint32_t>(seed) + 0x9E3779B9u);
   k = mix32(k ^ static_cast<uint32_t>(seed >> 32));
@@ -166,21 +166,40 @@ IADMM_DEV bool ordinary_codes(uint32_t m, uint32_t v) {  // no NaN (m & 127 = 12
   const uint32_t a = (m & 0x7F7F7F7Fu) + 0x01010101u, b = ((v & 0x7F7F7F7Fu) + 0x01010101u) & v;
   return ((a | b) & 0x80808080u) == 0u;
 }
+// Byte J of a word, moved to bits 20..27 (with its sign above, for m): one instruction each.
+template <int J> IADMM_DEV uint32_t byte_up(uint32_t q) {
+  uint32_t r;
+  const uint32_t by = 20;
+  if constexpr (J == 0) asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_0" : "=v"(r) : "v"(by), "v"(q));
+  if constexpr (J == 1) asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_1" : "=v"(r) : "v"(by), "v"(q));
+  if constexpr (J == 2) asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_2" : "=v"(r) : "v"(by), "v"(q));
+  if constexpr (J == 3) asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_3" : "=v"(r) : "v"(by), "v"(q));
+  return r;
+}
+template <int J> IADMM_DEV uint32_t signed_byte_up(uint32_t q) {
+  uint32_t r;
+  const uint32_t by = 20;
+  if constexpr (J == 0) asm("v_lshlrev_b32_sdwa %0, %1, sext(%2) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_0" : "=v"(r) : "v"(by), "v"(q));
+  if constexpr (J == 1) asm("v_lshlrev_b32_sdwa %0, %1, sext(%2) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_1" : "=v"(r) : "v"(by), "v"(q));
+  if constexpr (J == 2) asm("v_lshlrev_b32_sdwa %0, %1, sext(%2) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_2" : "=v"(r) : "v"(by), "v"(q));
+  if constexpr (J == 3) asm("v_lshlrev_b32_sdwa %0, %1, sext(%2) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_3" : "=v"(r) : "v"(by), "v"(q));
+  return r;
+}
 template <int J> IADMM_DEV float decode_m_of(uint32_t q, float scale) {
-  const int t = static_cast<int>(q << (24 - 8 * J));  // the sign in place; shifted on, it is above the magnitude
-  return bits_f(static_cast<uint32_t>(t >> 4) & 0x87F00000u) * scale;
+  return bits_f(signed_byte_up<J>(q) & 0x87F00000u) * scale;
 }
-template <int J> IADMM_DEV float decode_v_of(uint32_t q, float scale) {
-  return bits_f((q >> 8 * J & 255u) << 20) * scale;
-}
+template <int J> IADMM_DEV float decode_v_of(uint32_t q, float scale) { return bits_f(byte_up<J>(q)) * scale; }
 // The code in the top byte (the blocks' exponents keep it below NaN's and infinity's).
 IADMM_DEV uint32_t encode_m_top(float m, float scale, uint32_t bits) {
   const uint32_t a = (__float_as_uint(fabsf(m) * scale) + (bits >> 20 << 8)) << 4;
-  return (__float_as_uint(m) & 0x80000000u) | a;
+  return __float_as_uint(copysignf(bits_f(a), m));
 }
+// The median lifts what is below the first code onto it, and leaves 0 (and what fp32 itself holds with less than 20
+// bits, below 2^-129) where it is: the scaled value is never above v.
 IADMM_DEV uint32_t encode_v_top(float v, float scale, uint32_t bits) {
-  const uint32_t a = __float_as_uint(v * scale) + (bits & 0xFFFFFu), one = 1u << 20;
-  return (v > 0.0f && a < one ? one : a) << 4;
+  const uint32_t x = __float_as_uint(v * scale), y = __float_as_uint(v), one = 1u << 20;
+  const uint32_t lo = x < one ? x : one, hi = x < one ? one : x, mid = hi < y ? hi : y;
+  return ((lo > mid ? lo : mid) + (bits & 0xFFFFFu)) << 4;  // (the median of x, y and one)
 }
 IADMM_DEV uint32_t top_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   const uint32_t lo = __builtin_amdgcn_perm(b, a, 0x00000703u), hi = __builtin_amdgcn_perm(d, c, 0x07030000u);
@@ -259,7 +278,11 @@ IADMM_DEV void adam_wave(const AdamLaunch& a, const AdamTensor& t, const AdamSca
     const int64_t i = at + u * 256 + lane * 4, left = t.n - i;
     float fm[4], fv[4], np[4];
     uint32_t bits[4] = {0, 0, 0, 0};
-    const uint32_t place = static_cast<uint32_t>(i) + static_cast<uint32_t>(i >> 32) * 0x9E3779B9u;  // (i % 4 = 0: no carry)
+    // the element's place and the key, with mix32's first step: for four neighbours from i, a multiple of 4, they
+    // differ by an exclusive or with 0..3 alone
+    const uint32_t first = static_cast<uint32_t>(i) ^ static_cast<uint32_t>(i >> 32) * 0x9E3779B9u ^ s.key;
+    const uint32_t mixed = first ^ first >> 16;
+    bool odd = false;
     if constexpr (EIGHT) {
       const int em = __builtin_amdgcn_readfirstlane(old[2 * u]), ev = __builtin_amdgcn_readfirstlane(old[2 * u + 1]);
       if (em <= kFastM && ev <= kFastV && __all(ordinary_codes(cm[u], cv[u]))) {
@@ -271,6 +294,7 @@ IADMM_DEV void adam_wave(const AdamLaunch& a, const AdamTensor& t, const AdamSca
       } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j) fm[j] = decode_m(cm[u] >> 8 * j & 255u, em), fv[j] = decode_v(cv[u] >> 8 * j & 255u, ev);
+        odd = true;
       }
     } else {
 #pragma unroll
@@ -285,12 +309,12 @@ IADMM_DEV void adam_wave(const AdamLaunch& a, const AdamTensor& t, const AdamSca
       if constexpr (EIGHT) {
         // the hardware's root and reciprocal, 1 ulp each: with 8-bit moments the arithmetic takes as long as the
         // memory, and their correctly rounded forms are a third of it
-        const float d = __builtin_amdgcn_sqrtf(fv[j]) * s.ibc2 + a.eps;
-        np[j] = kept - s.step_size * (fm[j] * __builtin_amdgcn_rcpf(d));
+        const float d = fmaf(__builtin_amdgcn_sqrtf(fv[j]), s.ibc2, a.eps);
+        np[j] = fmaf(-s.step_size, fm[j] * __builtin_amdgcn_rcpf(d), kept);
       } else {
         np[j] = kept - s.step_size * (fm[j] / (sqrtf(fv[j]) * s.ibc2 + a.eps));
       }
-      if constexpr (EIGHT || sizeof(P) == 2) bits[j] = mix32((place + j) ^ s.key);
+      if constexpr (EIGHT || sizeof(P) == 2) bits[j] = mix32_rest(mixed ^ static_cast<uint32_t>(j));
     }
     if constexpr (!EIGHT) {
       store_quad<FULL>(p + i, new_params<P, true>(np, bits), left);
@@ -299,16 +323,15 @@ IADMM_DEV void adam_wave(const AdamLaunch& a, const AdamTensor& t, const AdamSca
       store_quad<FULL>(m + i, qm[u], left);
       store_quad<FULL>(v + i, qv[u], left);
     } else {
-      uint32_t tm = 0, tv = 0;  // (elements behind the end are 0; v is never negative)
+      // (elements behind the end are 0; v is never negative.  NaN is none of tm's: where a gradient made m infinite or NaN,
+      // v is so too, and where the state had it, `odd` says so)
+      uint32_t tm = __float_as_uint(fmaxf(fmaxf(fabsf(fm[0]), fabsf(fm[1])), fmaxf(fabsf(fm[2]), fabsf(fm[3]))));
+      uint32_t tv = 0;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t bm = __float_as_uint(fm[j]) & 0x7FFFFFFFu, bv = __float_as_uint(fv[j]);
-        tm = bm > tm ? bm : tm;
-        tv = bv > tv ? bv : tv;
-      }
+      for (int j = 0; j < 4; ++j) tv = __float_as_uint(fv[j]) > tv ? __float_as_uint(fv[j]) : tv;
       wave_umax(tm, tv);
       int ne = block_exponent(tm, 8, -117, 120), nv = block_exponent(tv, 0, -93, 127);
-      if (tm < 0x7F800000u && tv < 0x7F800000u && ne <= kFastM && nv <= kFastV) {
+      if (!odd && tv < 0x7F800000u && ne <= kFastM && nv <= kFastV) {
         store_quad<FULL>(p + i, new_params<P, false>(np, bits), left);
         const float sm = pow2(-ne - 120), sv = pow2(-nv - 96);
         uint32_t tops[4];

@@ -459,7 +459,7 @@ def test_offsets_beyond_32_bits():
         k = mix(k)
         key = mix(mix((int(k) + 1) & 0xFFFFFFFF))
         with np.errstate(over="ignore"):
-            low = (idx & np.uint64(0xFFFFFFFF)).astype(np.uint32) + (idx >> np.uint64(32)).astype(np.uint32) * np.uint32(0x9E3779B9)
+            low = (idx & np.uint64(0xFFFFFFFF)).astype(np.uint32) ^ (idx >> np.uint64(32)).astype(np.uint32) * np.uint32(0x9E3779B9)
         bits = mix(low ^ key)
         m = np.zeros(z - a, np.float32)
         p = np.full(z - a, float(torch.tensor(0.1).bfloat16()), np.float32)
