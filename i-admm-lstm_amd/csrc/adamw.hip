@@ -21,13 +21,15 @@
 // is for good, rounding at random keeps its mean.  The same holds for bf16 parameters (half a step is 2^-9 of
 // the value, lr is 1e-4).  A v that is not zero does not become zero: m / sqrt(v) would jump.
 // The 32 bits belong to (seed, step, the tensor's place, the element's place), so a run can be repeated.
+#include <string.h>
+
 #include <type_traits>
 
 #include "common.h"
 
 namespace iadmm {
 
-constexpr int kPer = 48;          // tensors of a launch: they travel in its arguments (3.5 KB of 4)
+constexpr int kPer = 48;          // tensors that travel in a launch's arguments (3.5 KB of 4)
 constexpr int kBlock8 = 256;      // elements under one pair of exponents
 constexpr int kNormPer = 128, kNormBlocks = 1024;
 
@@ -38,18 +40,28 @@ struct AdamTensor {
   const void* g;
   void *m, *v, *e;
   int64_t n;
-  float step_size, ibc2;
-  uint32_t key;
-  uint32_t first;  // its first workgroup
-  int flags, slot;
+  float step_size, ibc2, decay;  // lr / (1 - b1^t), 1 / sqrt(1 - b2^t), 1 - lr wd
+  uint32_t key;                  // (its slot, on the way to adam_place_kernel)
+  uint32_t first;                // its first workgroup
+  int flags;
 };
+static_assert(sizeof(AdamTensor) == 72, "words below");
 
+struct AdamCommon {
+  const float* norm;  // or null
+  float b1, ob1, b2, ob2, eps, max_norm;
+  int count;
+};
+// The tensors in the arguments, or in a table in memory that adam_place_kernel wrote: for more than kPer of them (216
+// tensors of 100 M bf16 elements with 8-bit moments: 224 us, with five launches, each with a start and an end of its own,
+// 262) and where the device counts (16 tensors of 2.6 M fp32 elements: 18.8 us; from the arguments 16.3).
 struct AdamLaunch {
   AdamTensor t[kPer];
-  const float* norm;     // or null
-  const float4* table;   // step size, 1 / sqrt(1 - b2^t), 1 - lr wd, key of each tensor, or null: those of t
-  float decay, b1, ob1, b2, ob2, eps, max_norm;
-  int count;
+  AdamCommon c;
+};
+struct AdamTable {
+  const AdamTensor* t;
+  AdamCommon c;
 };
 
 // 32 well-mixed bits of 32: two odd multipliers between shifts, chosen by search for the least bias of any
@@ -206,23 +218,19 @@ IADMM_DEV uint32_t top_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   return __builtin_amdgcn_perm(hi, lo, 0x07060100u);
 }
 
-// Which of the launch's tensors this workgroup serves: the last whose first workgroup is not behind it.
-template <typename L> IADMM_DEV int find_tensor(const L& a, uint32_t block) {
-  int at = 0;
-  for (int k = threadIdx.x % kWave; k < a.count; k += kWave)
-    if (a.t[k].first <= block) at = k;
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) {
-    const int w = __shfl_xor(at, o, kWave);
-    at = w > at ? w : at;
+// The last of `count` tensors whose first workgroup is not behind this one: 64 at a time from a stride apart, closer.
+// (An empty tensor has its successor's first workgroup, and is never the last with it.)
+template <typename T> IADMM_DEV int find_tensor(const T& t, int count, uint32_t block) {
+  const int lane = threadIdx.x % kWave;
+  int at = 0, n = count;
+  for (;;) {
+    const int stride = (n + kWave - 1) / kWave, k = lane * stride;
+    const int reached = __popcll(__ballot(k < n && t[at + (k < n ? k : 0)].first <= block));
+    at += (reached - 1) * stride;
+    if (stride == 1) return __builtin_amdgcn_readfirstlane(at);
+    n = n - (reached - 1) * stride < stride ? n - (reached - 1) * stride : stride;
   }
-  return __builtin_amdgcn_readfirstlane(at);
 }
-
-struct AdamScalars {
-  float step_size, ibc2, decay, clip;
-  uint32_t key;
-};
 
 // The new parameters of four elements; `bits` are 0 for fp32.  SAFE: NaN keeps its bits (random ones added to a payload
 // of ones would carry into the sign; where the moments are finite, a NaN is a bf16 parameter's own, with lower bits 0).
@@ -247,7 +255,7 @@ template <typename P, bool SAFE> IADMM_DEV Quad<P> new_params(const float (&np)[
 
 // QUADS x 256 elements per wave.
 template <typename P, typename G, bool EIGHT, int QUADS, bool FULL>
-IADMM_DEV void adam_wave(const AdamLaunch& a, const AdamTensor& t, const AdamScalars& s, int64_t at) {
+IADMM_DEV void adam_wave(const AdamCommon& a, const AdamTensor& t, float clip, int64_t at) {
   const int lane = threadIdx.x % kWave;
   P* p = static_cast<P*>(t.p);
   const G* g = static_cast<const G*>(t.g);
@@ -280,7 +288,7 @@ IADMM_DEV void adam_wave(const AdamLaunch& a, const AdamTensor& t, const AdamSca
     uint32_t bits[4] = {0, 0, 0, 0};
     // the element's place and the key, with mix32's first step: for four neighbours from i, a multiple of 4, they
     // differ by an exclusive or with 0..3 alone
-    const uint32_t first = static_cast<uint32_t>(i) ^ static_cast<uint32_t>(i >> 32) * 0x9E3779B9u ^ s.key;
+    const uint32_t first = static_cast<uint32_t>(i) ^ static_cast<uint32_t>(i >> 32) * 0x9E3779B9u ^ t.key;
     const uint32_t mixed = first ^ first >> 16;
     bool odd = false;
     if constexpr (EIGHT) {
@@ -302,17 +310,17 @@ IADMM_DEV void adam_wave(const AdamLaunch& a, const AdamTensor& t, const AdamSca
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float gr = static_cast<float>(qg[u].v[j]) * s.clip;
+      const float gr = static_cast<float>(qg[u].v[j]) * clip;
       fm[j] = a.b1 * fm[j] + a.ob1 * gr;
       fv[j] = a.b2 * fv[j] + a.ob2 * (gr * gr);
-      const float kept = static_cast<float>(qp[u].v[j]) * s.decay;
+      const float kept = static_cast<float>(qp[u].v[j]) * t.decay;
       if constexpr (EIGHT) {
         // the hardware's root and reciprocal, 1 ulp each: with 8-bit moments the arithmetic takes as long as the
         // memory, and their correctly rounded forms are a third of it
-        const float d = fmaf(__builtin_amdgcn_sqrtf(fv[j]), s.ibc2, a.eps);
-        np[j] = fmaf(-s.step_size, fm[j] * __builtin_amdgcn_rcpf(d), kept);
+        const float d = fmaf(__builtin_amdgcn_sqrtf(fv[j]), t.ibc2, a.eps);
+        np[j] = fmaf(-t.step_size, fm[j] * __builtin_amdgcn_rcpf(d), kept);
       } else {
-        np[j] = kept - s.step_size * (fm[j] / (sqrtf(fv[j]) * s.ibc2 + a.eps));
+        np[j] = kept - t.step_size * (fm[j] / (sqrtf(fv[j]) * t.ibc2 + a.eps));
       }
       if constexpr (EIGHT || sizeof(P) == 2) bits[j] = mix32_rest(mixed ^ static_cast<uint32_t>(j));
     }
@@ -372,60 +380,70 @@ IADMM_DEV void adam_wave(const AdamLaunch& a, const AdamTensor& t, const AdamSca
 }
 
 template <typename P, typename G, bool EIGHT, int QUADS>
-IADMM_DEV void adam_chunk(const AdamLaunch& a, const AdamTensor& t, const AdamScalars& s) {
+IADMM_DEV void adam_chunk(const AdamCommon& a, const AdamTensor& t, float clip) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int64_t at = (static_cast<int64_t>(blockIdx.x - t.first) * 4 + wave) * (QUADS * 256);
   if (at + QUADS * 256 <= t.n) {
-    adam_wave<P, G, EIGHT, QUADS, true>(a, t, s, at);
+    adam_wave<P, G, EIGHT, QUADS, true>(a, t, clip, at);
   } else {
     for (int u = 0; u < QUADS; ++u)
-      if (at + u * 256 < t.n) adam_wave<P, G, EIGHT, 1, false>(a, t, s, at + u * 256);
+      if (at + u * 256 < t.n) adam_wave<P, G, EIGHT, 1, false>(a, t, clip, at + u * 256);
   }
 }
 
-template <bool EIGHT, int QUADS> __global__ void __launch_bounds__(256) adam_kernel(const AdamLaunch a) {
-  const int k = find_tensor(a, blockIdx.x);
-  const AdamTensor& t = a.t[k];
-  AdamScalars s{t.step_size, t.ibc2, a.decay, 1.0f, t.key};
-  if (a.table) {
-    const float4 f = a.table[k];
-    s.step_size = f.x;
-    s.ibc2 = f.y;
-    s.decay = f.z;
-    s.key = __float_as_uint(f.w);
-  }
+template <bool EIGHT, int QUADS> IADMM_DEV void adam_any(const AdamCommon& a, const AdamTensor& t) {
+  float clip = 1.0f;
   if (a.norm) {
     const float c = a.max_norm / (*a.norm + 1e-6f);
-    s.clip = c > 1.0f ? 1.0f : c;  // (a norm that is NaN reaches every parameter)
+    clip = c > 1.0f ? 1.0f : c;  // (a norm that is NaN reaches every parameter)
   }
   switch (t.flags) {
-    case 0: adam_chunk<float, float, EIGHT, QUADS>(a, t, s); break;
-    case kHalfG: adam_chunk<float, __bf16, EIGHT, QUADS>(a, t, s); break;
-    case kHalfP: adam_chunk<__bf16, float, EIGHT, QUADS>(a, t, s); break;
-    default: adam_chunk<__bf16, __bf16, EIGHT, QUADS>(a, t, s); break;
+    case 0: adam_chunk<float, float, EIGHT, QUADS>(a, t, clip); break;
+    case kHalfG: adam_chunk<float, __bf16, EIGHT, QUADS>(a, t, clip); break;
+    case kHalfP: adam_chunk<__bf16, float, EIGHT, QUADS>(a, t, clip); break;
+    default: adam_chunk<__bf16, __bf16, EIGHT, QUADS>(a, t, clip); break;
   }
 }
+template <bool EIGHT, int QUADS> __global__ void __launch_bounds__(256) adam_kernel(const AdamLaunch a) {
+  adam_any<EIGHT, QUADS>(a.c, a.t[find_tensor(a.t, a.c.count, blockIdx.x)]);
+}
+template <bool EIGHT, int QUADS> __global__ void __launch_bounds__(256) adam_table_kernel(const AdamTable a) {
+  const AdamTensor* from = a.t + find_tensor(a.t, a.c.count, blockIdx.x);
+  int w[sizeof(AdamTensor) / 4];  // the same for the workgroup: scalars
+  __builtin_memcpy(w, from, sizeof(w));
+#pragma unroll
+  for (unsigned i = 0; i < sizeof(w) / 4; ++i) w[i] = __builtin_amdgcn_readfirstlane(w[i]);
+  AdamTensor t;
+  __builtin_memcpy(&t, w, sizeof(w));
+  adam_any<EIGHT, QUADS>(a.c, t);
+}
 
-// Steps that live on the device (a captured step has to count by itself): counts, and writes what the
-// parameters' kernel needs of the count.
-struct AdamCount {
-  int slot[kPer];
+// Writes tensors into the table; where the steps are counted on the device (a captured step has to count by itself),
+// counts, and works out what depends on the count.
+struct AdamPlace {
+  AdamTensor t[kPer];
+  AdamTensor* to;
   int64_t* steps;
   const float* lr;
   double lr_host, b1, b2, decay;
   uint64_t seed;
-  float4* table;
   int count;
 };
-__global__ void adam_count_kernel(const AdamCount a) {
+__global__ void adam_place_kernel(const AdamPlace a) {
   const int k = threadIdx.x;
   if (k >= a.count) return;
-  const int64_t step = a.steps[a.slot[k]] + 1;
-  a.steps[a.slot[k]] = step;
-  const double lr = a.lr ? static_cast<double>(*a.lr) : a.lr_host, t = static_cast<double>(step);
-  a.table[k] = make_float4(static_cast<float>(lr / (1.0 - pow(a.b1, t))), static_cast<float>(1.0 / sqrt(1.0 - pow(a.b2, t))),
-                           static_cast<float>(1.0 - lr * a.decay),
-                           __uint_as_float(step_key(a.seed, static_cast<uint64_t>(step), a.slot[k])));
+  AdamTensor d = a.t[k];
+  if (a.steps) {
+    const int slot = static_cast<int>(d.key);
+    const int64_t step = a.steps[slot] + 1;
+    a.steps[slot] = step;
+    const double lr = a.lr ? static_cast<double>(*a.lr) : a.lr_host, t = static_cast<double>(step);
+    d.step_size = static_cast<float>(lr / (1.0 - pow(a.b1, t)));
+    d.ibc2 = static_cast<float>(1.0 / sqrt(1.0 - pow(a.b2, t)));
+    d.decay = static_cast<float>(1.0 - lr * a.decay);
+    d.key = step_key(a.seed, static_cast<uint64_t>(step), slot);
+  }
+  a.to[k] = d;
 }
 
 // The codes' values, 1024 per wave.
@@ -519,7 +537,7 @@ template <int QUADS> __global__ void __launch_bounds__(256) norm_kernel(const No
   // a run of neighbouring chunks, so that the tensor is looked for once
   uint32_t c = static_cast<uint32_t>(static_cast<uint64_t>(a.chunks) * blockIdx.x / gridDim.x);
   const uint32_t end = static_cast<uint32_t>(static_cast<uint64_t>(a.chunks) * (blockIdx.x + 1) / gridDim.x);
-  int k = find_tensor(a, c);
+  int k = find_tensor(a.t, a.count, c);
   double s = 0.0;
   for (; c < end; ++c) {
     while (k + 1 < a.count && a.t[k + 1].first <= c) ++k;
@@ -542,12 +560,11 @@ __global__ void __launch_bounds__(1024) norm_end_kernel(const double* part, int 
 // Workgroups take 2048 elements at a time up to this many in all, 8192 above: 168 000 of them 7.1 us against 7.7 (with the
 // last sum's launch), 2.6 M 8.2 against 8.0.
 constexpr int64_t kNormSmall = int64_t{1} << 19;
-template <int QUADS> static int launch_norm(NormLaunch& a, hipStream_t st) {  // the workgroups, or an error
+template <int QUADS> static int launch_norm(NormLaunch& a, hipStream_t st) {  // gives its workgroups
   uint64_t chunks = 0;
   for (int k = 0; k < a.count; ++k) {
     a.t[k].first = static_cast<uint32_t>(chunks);
     chunks += (static_cast<uint64_t>(a.t[k].n) + QUADS * 1024 - 1) / (QUADS * 1024);
-    if (chunks > 0x7FFFFFFFu) return IADMM_E_SIZE;
   }
   a.chunks = static_cast<uint32_t>(chunks);
   const int blocks = chunks < kNormBlocks ? static_cast<int>(chunks) : kNormBlocks;
@@ -558,16 +575,12 @@ template <int QUADS> static int launch_norm(NormLaunch& a, hipStream_t st) {  //
 // Workgroups of 1024 elements up to this many in all, of 4096 above: 168 000 of them 7.9 us against 8.9 (with the
 // counting launch), 2.6 M 17.9 against 16.6.
 constexpr int64_t kAdamSmall = int64_t{1} << 19;
-template <bool EIGHT, int QUADS> static int launch_adam(AdamLaunch& a, hipStream_t st) {
-  uint64_t blocks = 0;
-  for (int k = 0; k < a.count; ++k) {
-    a.t[k].first = static_cast<uint32_t>(blocks);
-    blocks += (static_cast<uint64_t>(a.t[k].n) + 1024 * QUADS - 1) / (1024 * QUADS);
-  }
-  if (blocks > 0xFFFFFFu) return IADMM_E_SIZE;  // 2^32 threads
-  hipLaunchKernelGGL((adam_kernel<EIGHT, QUADS>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, st, a);
-  IADMM_CHECK_LAUNCH();
-  return IADMM_OK;
+template <bool EIGHT, int QUADS> static void launch_adam(const AdamLaunch& a, const AdamTensor* table, unsigned blocks,
+                                                       hipStream_t st) {
+  if (table)
+    hipLaunchKernelGGL((adam_table_kernel<EIGHT, QUADS>), dim3(blocks), dim3(256), 0, st, AdamTable{table, a.c});
+  else
+    hipLaunchKernelGGL((adam_kernel<EIGHT, QUADS>), dim3(blocks), dim3(256), 0, st, a);
 }
 
 }  // namespace iadmm
@@ -583,10 +596,11 @@ extern "C" int iadmm_grad_norm(int64_t count, const iadmm_grad_tensor* grads, fl
                                void* stream) {
   if (count < 0 || !norm || (count > 0 && (!grads || !ws)) || ws_bytes < iadmm_grad_norm_ws_bytes(count)) return IADMM_E_ARG;
   if (!aligned16(ws)) return IADMM_E_ALIGN;
+  int64_t all = 0;
   for (int64_t i = 0; i < count; ++i) {
     if (grads[i].n < 0 || (grads[i].n > 0 && !grads[i].g) || (grads[i].dtype != IADMM_F32 && grads[i].dtype != IADMM_BF16))
       return IADMM_E_ARG;
-    if (grads[i].n > (int64_t{1} << 40)) return IADMM_E_SIZE;
+    if (grads[i].n > (int64_t{1} << 40) || (all += grads[i].n) > (int64_t{1} << 40)) return IADMM_E_SIZE;
   }
   hipStream_t st = static_cast<hipStream_t>(stream);
   double* part = static_cast<double*>(ws);
@@ -602,7 +616,6 @@ extern "C" int iadmm_grad_norm(int64_t count, const iadmm_grad_tensor* grads, fl
     if (a.count > 0 && (a.count == kNormPer || i == count - 1)) {
       a.part = part + parts;
       const int blocks = total <= kNormSmall ? launch_norm<2>(a, st) : launch_norm<8>(a, st);
-      if (blocks < 0) return blocks;
       IADMM_CHECK_LAUNCH();
       parts += blocks;
       a.count = 0;
@@ -614,65 +627,75 @@ extern "C" int iadmm_grad_norm(int64_t count, const iadmm_grad_tensor* grads, fl
   return IADMM_OK;
 }
 
-extern "C" int64_t iadmm_adamw_ws_bytes(int64_t count) { return count <= 0 ? 0 : count * static_cast<int64_t>(sizeof(float4)); }
+extern "C" int64_t iadmm_adamw_ws_bytes(int64_t count) {
+  return count <= 0 ? 0 : count * static_cast<int64_t>(sizeof(AdamTensor));
+}
 
 extern "C" int iadmm_adamw_step(int64_t count, const iadmm_adamw_tensor* tensors, int state_bits, double lr, const float* lr_dev,
                                 double beta1, double beta2, double eps, double weight_decay, const float* norm,
                                 double max_norm, uint64_t seed, int64_t* steps_dev, void* ws, int64_t ws_bytes,
                                 void* stream) {
-  const bool eight = state_bits == 8;
+  const bool eight = state_bits == 8, table = steps_dev || count > kPer;
   if (count < 0 || (count > 0 && !tensors) || (!eight && state_bits != 32)) return IADMM_E_ARG;
   if (!(lr >= 0.0) || !(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0) || !(eps >= 0.0) ||
       !(weight_decay >= 0.0) || (norm && !(max_norm > 0.0)) || (lr_dev && !steps_dev))
     return IADMM_E_ARG;
-  if (steps_dev && (!ws || ws_bytes < iadmm_adamw_ws_bytes(count))) return IADMM_E_ARG;
-  if (steps_dev && !aligned16(ws)) return IADMM_E_ALIGN;
+  if (table && (!ws || ws_bytes < iadmm_adamw_ws_bytes(count))) return IADMM_E_ARG;
+  if (table && !aligned16(ws)) return IADMM_E_ALIGN;
+  if (count > 0x7FFFFFFF) return IADMM_E_SIZE;
+  int64_t total = 0;
   for (int64_t i = 0; i < count; ++i) {
     const iadmm_adamw_tensor& t = tensors[i];
     if (t.n < 0 || t.slot < 0 || (t.n > 0 && (!t.p || !t.g || !t.m || !t.v || (eight && !t.e))) ||
         (!steps_dev && t.step < 1) || (t.dtype != IADMM_F32 && t.dtype != IADMM_BF16) ||
         (t.gdtype != IADMM_F32 && t.gdtype != IADMM_BF16))
       return IADMM_E_ARG;
-    if (t.n > (int64_t{1} << 40)) return IADMM_E_SIZE;
+    if (t.n > (int64_t{1} << 36) || (total += t.n) > (int64_t{1} << 36)) return IADMM_E_SIZE;
   }
+  const int64_t each = total <= kAdamSmall ? 1024 : 4096;
+  uint64_t blocks = 0;
+  for (int64_t i = 0; i < count; ++i) blocks += (static_cast<uint64_t>(tensors[i].n) + each - 1) / each;
+  if (blocks > 0xFFFFFFu) return IADMM_E_SIZE;  // 2^32 threads
   hipStream_t st = static_cast<hipStream_t>(stream);
-  float4* table = static_cast<float4*>(ws);
-  for (int64_t from = 0; from < count; from += kPer) {
-    AdamLaunch a;
-    AdamCount c;
-    const int64_t part = count - from < kPer ? count - from : kPer;
-    a.count = 0;
-    int64_t total = 0;
-    for (int64_t i = from; i < from + part; ++i) {
-      const iadmm_adamw_tensor& t = tensors[i];
-      c.slot[i - from] = t.slot;
-      if (t.n == 0 && !steps_dev) continue;  // (with counts on the device an empty tensor counts too)
-      AdamTensor& d = a.t[a.count++];
-      d.p = t.p, d.g = t.g, d.m = t.m, d.v = t.v, d.e = t.e, d.n = t.n, d.slot = t.slot;
-      d.flags = (t.dtype == IADMM_BF16 ? kHalfP : 0) | (t.gdtype == IADMM_BF16 ? kHalfG : 0);
-      const double k = static_cast<double>(t.step);
-      d.step_size = steps_dev ? 0.0f : static_cast<float>(lr / (1.0 - pow(beta1, k)));
-      d.ibc2 = steps_dev ? 0.0f : static_cast<float>(1.0 / sqrt(1.0 - pow(beta2, k)));
-      d.key = steps_dev ? 0u : step_key(seed, static_cast<uint64_t>(t.step), t.slot);
-      total += t.n;
+  AdamPlace a{};
+  a.steps = steps_dev, a.lr = lr_dev, a.lr_host = lr, a.b1 = beta1, a.b2 = beta2, a.decay = weight_decay, a.seed = seed;
+  a.to = static_cast<AdamTensor*>(ws);
+  int64_t step = 0;
+  float step_size = 0.0f, ibc2 = 0.0f;
+  uint32_t first = 0;
+  for (int64_t i = 0; i < count; ++i) {
+    const iadmm_adamw_tensor& t = tensors[i];
+    if (!steps_dev && t.step != step) {
+      step = t.step;
+      step_size = static_cast<float>(lr / (1.0 - pow(beta1, static_cast<double>(step))));
+      ibc2 = static_cast<float>(1.0 / sqrt(1.0 - pow(beta2, static_cast<double>(step))));
     }
-    a.norm = norm, a.max_norm = static_cast<float>(max_norm);
-    a.table = steps_dev ? table + from : nullptr;
-    a.decay = static_cast<float>(1.0 - lr * weight_decay), a.eps = static_cast<float>(eps);
-    a.b1 = static_cast<float>(beta1), a.ob1 = static_cast<float>(1.0 - beta1);
-    a.b2 = static_cast<float>(beta2), a.ob2 = static_cast<float>(1.0 - beta2);
-    if (steps_dev) {
-      c.steps = steps_dev, c.lr = lr_dev, c.lr_host = lr, c.b1 = beta1, c.b2 = beta2, c.decay = weight_decay;
-      c.seed = seed, c.table = table + from, c.count = static_cast<int>(part);
-      hipLaunchKernelGGL(adam_count_kernel, dim3(1), dim3(64), 0, st, c);
+    AdamTensor& d = a.t[a.count++];
+    d.p = t.p, d.g = t.g, d.m = t.m, d.v = t.v, d.e = t.e, d.n = t.n, d.first = first;
+    d.flags = (t.dtype == IADMM_BF16 ? kHalfP : 0) | (t.gdtype == IADMM_BF16 ? kHalfG : 0);
+    d.step_size = step_size, d.ibc2 = ibc2, d.decay = static_cast<float>(1.0 - lr * weight_decay);
+    d.key = steps_dev ? static_cast<uint32_t>(t.slot) : step_key(seed, static_cast<uint64_t>(t.step), t.slot);
+    first += static_cast<uint32_t>((t.n + each - 1) / each);
+    if (table && (a.count == kPer || i == count - 1)) {
+      hipLaunchKernelGGL(adam_place_kernel, dim3(1), dim3(64), 0, st, a);
       IADMM_CHECK_LAUNCH();
+      a.to += a.count;
+      a.count = 0;
     }
-    if (total == 0) continue;
-    const bool small = total <= kAdamSmall;
-    const int rc = eight ? (small ? launch_adam<true, 1>(a, st) : launch_adam<true, 4>(a, st))
-                         : (small ? launch_adam<false, 1>(a, st) : launch_adam<false, 4>(a, st));
-    if (rc) return rc;
   }
+  if (blocks == 0) return IADMM_OK;
+  AdamLaunch l;
+  if (!table) memcpy(l.t, a.t, sizeof(l.t));
+  l.c = AdamCommon{norm, static_cast<float>(beta1), static_cast<float>(1.0 - beta1), static_cast<float>(beta2),
+                   static_cast<float>(1.0 - beta2), static_cast<float>(eps), static_cast<float>(max_norm),
+                   static_cast<int>(count)};
+  const AdamTensor* in = table ? static_cast<const AdamTensor*>(ws) : nullptr;
+  const unsigned n = static_cast<unsigned>(blocks);
+  if (eight && each == 1024) launch_adam<true, 1>(l, in, n, st);
+  else if (eight) launch_adam<true, 4>(l, in, n, st);
+  else if (each == 1024) launch_adam<false, 1>(l, in, n, st);
+  else launch_adam<false, 4>(l, in, n, st);
+  IADMM_CHECK_LAUNCH();
   return IADMM_OK;
 }
 

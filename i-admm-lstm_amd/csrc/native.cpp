@@ -427,9 +427,9 @@ PyObject* py_adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
   std::sort(held.begin(), held.end());
   TORCH_CHECK_VALUE(std::adjacent_find(held.begin(), held.end()) == held.end(),
                     "a parameter or its state is in the lists twice");
-  const int64_t many = static_cast<int64_t>(rec.size()), bytes = counted ? abi.adamw_ws_bytes(many) : 0;
+  const int64_t many = static_cast<int64_t>(rec.size()), bytes = abi.adamw_ws_bytes(many);
   const at::AutoGradMode off(false);
-  Tensor ws = counted ? f32_on(p.t[0], {bytes / 4}) : Tensor();
+  Tensor ws = counted || many > 48 ? f32_on(p.t[0], {bytes / 4}) : Tensor();  // (include/iadmm.h: when it is used)
   const c10::DeviceGuard guard(p.device);
   done("iadmm_adamw_step",
        abi.adamw_step(many, rec.data(), eight ? 8 : 32, lr, lr_dev.defined() ? lr_dev.const_data_ptr<float>() : nullptr, b1, b2,

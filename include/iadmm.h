@@ -394,7 +394,7 @@ int iadmm_layer_norm_bwd(int64_t rows, int64_t cols, int dtype, int wdtype, cons
  *     or IADMM_BF16.  No two tensors of a call may overlap.
  *     step: the step that this call makes, counted from 1; or, with steps_dev, steps_dev[slot] is raised by
  *     1 and used (a captured call then counts its replays); lr_dev (needs steps_dev), where not NULL,
- *     replaces lr.  ws: iadmm_adamw_ws_bytes(count) bytes, 16-B aligned, with steps_dev only.
+ *     replaces lr.  ws: iadmm_adamw_ws_bytes(count) bytes, 16-B aligned, with steps_dev or more than 48 tensors.
  *   iadmm_adamw_decode8: the values of n 8-bit codes, as fp32 or bf16 (both hold them exactly down to
  *     2^-126; a moment that overflowed is NaN for m, infinity for v). */
 typedef struct { const void* g; int64_t n; int64_t dtype; } iadmm_grad_tensor;

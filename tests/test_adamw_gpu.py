@@ -237,6 +237,23 @@ def test_many_tensors_and_missing_gradients(eight):
             assert all(torch.equal(a, b) for a, b in zip(L, K))
 
 
+@pytest.mark.parametrize("count", [48, 49, 64, 65, 4096, 4097, 9001])
+def test_long_lists(count):
+    """Every tensor of a list of any length is found, by its own workgroups: 1 to 3000 elements each, some empty."""
+    from iadmm import ops
+    sizes = np.array([(i * 7919) % 11 if i % 50 else (i * 31) % 3000 for i in range(count)])
+    starts = np.concatenate([[0], np.cumsum(sizes)])
+    n = int(starts[-1])
+    g = torch.Generator(device="cuda").manual_seed(count)
+    p, m = (torch.randn(n, device="cuda", generator=g) for _ in range(2))
+    gr, v = 1e-2 * torch.randn(n, device="cuda", generator=g), torch.rand(n, device="cuda", generator=g)
+    cut = lambda t: [t[a:z] for a, z in zip(starts[:-1].tolist(), starts[1:].tolist())]  # noqa: E731
+    want, up, wm, wv = step32(*(to_np(t) for t in (p, gr, m, v)), 5, 1e-3, (0.9, 0.999), 1e-8, 0.01)
+    ops.adamw_step(cut(p), cut(gr), cut(m), cut(v), 5, lr=1e-3)
+    check_params(p, want, up, None)
+    assert np.array_equal(to_np(m), wm) and np.array_equal(to_np(v), wv)
+
+
 def test_nothing_beside_a_tensor_is_written():
     from iadmm import ops
     for eight in (False, True):

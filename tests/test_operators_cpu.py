@@ -54,10 +54,12 @@ def test_adamw_arguments():
         refused("bad argument", f, *step_args(rec))
     refused("bad argument", f, *step_args(record(e=0), bits=8))
     refused("size beyond", f, *step_args(record(n=(1 << 40) + 1)))
+    refused("size beyond", f, *step_args(record(n=1 << 36) + record(n=1)))
+    refused("bad argument", f, *step_args(sum((record() for _ in range(49)), array.array("q"))))  # no workspace
     for kw in (dict(bits=16), dict(lr=-1.0), dict(lr=nan), dict(b1=1.0), dict(b2=nan), dict(eps=-1.0), dict(wd=-0.1),
-               dict(norm=16, most=0.0), dict(lr_dev=16), dict(steps=16), dict(steps=16, ws=16, nbytes=8)):
+               dict(norm=16, most=0.0), dict(lr_dev=16), dict(steps=16), dict(steps=16, ws=16, nbytes=64)):
         refused("bad argument", f, *step_args(record(), **kw))
-    refused("misaligned", f, *step_args(record(), steps=16, ws=20, nbytes=16))
+    refused("misaligned", f, *step_args(record(), steps=16, ws=20, nbytes=72))
     _abi.call(f, *step_args(record(p=0, g=0, m=0, v=0, n=0)))  # an empty tensor: nothing to do
     n = "iadmm_grad_norm"
     grad = array.array("q", [16, 4, 0])
