@@ -30,6 +30,7 @@
 namespace iadmm {
 
 constexpr int kPer = 48;          // tensors that travel in a launch's arguments (3.5 KB of 4)
+constexpr int kPlace = 55;        // tensors that adam_place_kernel's arguments carry (4 KB)
 constexpr int kBlock8 = 256;      // elements under one pair of exponents
 constexpr int kNormPer = 128, kNormBlocks = 1024;
 
@@ -421,7 +422,7 @@ template <bool EIGHT, int QUADS> __global__ void __launch_bounds__(256) adam_tab
 // Writes tensors into the table; where the steps are counted on the device (a captured step has to count by itself),
 // counts, and works out what depends on the count.
 struct AdamPlace {
-  AdamTensor t[kPer];
+  AdamTensor t[kPlace];
   AdamTensor* to;
   int64_t* steps;
   const float* lr;
@@ -429,6 +430,7 @@ struct AdamPlace {
   uint64_t seed;
   int count;
 };
+static_assert(sizeof(AdamPlace) <= 4096 && kPlace <= 64 && kPlace >= kPer, "a launch's arguments, one wave");
 __global__ void adam_place_kernel(const AdamPlace a) {
   const int k = threadIdx.x;
   if (k >= a.count) return;
@@ -676,7 +678,7 @@ extern "C" int iadmm_adamw_step(int64_t count, const iadmm_adamw_tensor* tensors
     d.step_size = step_size, d.ibc2 = ibc2, d.decay = static_cast<float>(1.0 - lr * weight_decay);
     d.key = steps_dev ? static_cast<uint32_t>(t.slot) : step_key(seed, static_cast<uint64_t>(t.step), t.slot);
     first += static_cast<uint32_t>((t.n + each - 1) / each);
-    if (table && (a.count == kPer || i == count - 1)) {
+    if (table && (a.count == kPlace || i == count - 1)) {
       hipLaunchKernelGGL(adam_place_kernel, dim3(1), dim3(64), 0, st, a);
       IADMM_CHECK_LAUNCH();
       a.to += a.count;
