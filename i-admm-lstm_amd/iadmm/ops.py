@@ -284,7 +284,7 @@ LU_RANK128 = 4    # include/iadmm.h IADMM_LU_RANK128 (the r04 rank-128 blocks wi
 
 
 class LuContext:
-    """An iadmm_lu_ctx: the look-ahead's two priority streams and four events, owned by the caller
+    """An iadmm_lu_ctx: the look-ahead's two streams and four events, owned by the caller
     (include/iadmm.h).  Made on the current device; destroyed with the object."""
 
     def __init__(self):

@@ -126,7 +126,7 @@ int iadmm_kkt_rhs(int64_t B, int64_t n, int64_t m, int64_t num_ineq, const float
  * nothing is allocated inside.
  * iadmm_lu_factor runs every launch in order on `stream`.  iadmm_lu_factor_ex with a context (N <= 36736)
  * factors the next block beside the rest of each trailing update (look-ahead) on the context's two
- * streams (high / low priority), forked from and joined back into `stream` on every path, errors
+ * streams, forked from and joined back into `stream` on every path, errors
  * included: the call stays asynchronous and ordered on `stream`, and the factors are bit for bit
  * those of iadmm_lu_factor.  Under stream capture (hipGraph) the call ignores the context and runs
  * every launch on `stream` (the cross-stream fork / join crashed the HIP 7.2 runtime at capture end).
