@@ -577,7 +577,7 @@ IADMM_DEV void cell_epi_load(const CellArgsT& a, int jt, int64_t rbase, int wave
   }
 }
 
-// Packed epilogue: unit pairs (jj, jj+1) go through v_pk_*_f32 together (common.h *_cell2).
+// Paired epilogue: unit pairs (jj, jj+1) go through the two-value forms together (common.h *_cell2).
 // sWp = the tile's Wx fields as [16 unit pairs][16 fields][2 units] (cell_fill_wpairs), so one
 // float4 holds two fields of both units of a pair.  The projection partial runs as two interleaved
 // sums (even / odd unit of each pair) added at the end.

@@ -33,9 +33,10 @@ IADMM_DEV float tmax(float a, float b) { return (a != a || b != b) ? __builtin_n
 IADMM_DEV float sigmoidf_(float x) { return 1.0f / (1.0f + expf(-x)); }
 
 // LSTM-cell transcendentals, branch-free (tools/mathcheck.hip measures them against fp64).  Each
-// has a scalar form and a packed two-lane form (v_pk_*_f32 for everything but the v_exp/v_rcp
-// transcendentals and the clamp) built from the SAME operation sequence, so both give bitwise
-// identical results; the cell epilogue runs the packed form, the training recompute the scalar.
+// has a scalar form and forms for two and four values built from the SAME operation sequence, so all give
+// bitwise identical results; the cell epilogue runs the wide forms, the training recompute the scalar.
+// (The wide forms were written for v_pk_*_f32; the Makefile has these off, and they compile to scalar
+// pairs that no longer wait for each other.)
 //   sigmoid: 1 / (1 + 2^(-x log2 e)) on v_exp_f32 + v_rcp_f32 (relative error ~|x| 2^-24: no
 //            cancellation anywhere)
 //   tanh:    x P(x^2) / Q(x^2), P of degree 6, Q of degree 3 in x^2, on |x| clamped to 7.9053

@@ -163,7 +163,7 @@ IADMM_DEV void cell_bwd_tile(const CellBwdArgs& a, int jt, int rt, float* dsm, f
 #pragma unroll
   for (int q = 0; q < 16; ++q) whp[q] = 0.f;
   if constexpr (VEC) {
-    // Packed epilogue: unit pairs through v_pk_*_f32 (the forward's gate values bit for bit:
+    // Paired epilogue: unit pairs through the two-value forms (the forward's gate values bit for bit:
     // same operations as cell_epi_compute_buf).  h % 4 == 0: a lane's 4 units are all valid or not.
     // Global accesses through buffer descriptors based at the workgroup's row panel, ranges ending
     // at its last valid row (rows past M read 0 / are dropped; a NULL dH' / dC' is an empty
