@@ -4,8 +4,13 @@
 //   m' = b1 m + (1 - b1) g',  v' = b2 v + (1 - b2) g'^2
 //   p' = p (1 - lr wd) - lr / (1 - b1^t) * m' / (sqrt(v') / sqrt(1 - b2^t) + eps)
 //
-// in fp32, each product and sum rounded by itself.  Bound: HBM, 28 bytes an element for fp32 parameters with
-// 32-bit moments, 16 with 8-bit ones, 10 for bf16 parameters and gradients with 8-bit moments.
+// in fp32, each product and sum rounded by itself (with 8-bit moments the parameters' last steps are fused).  Bound:
+// HBM, 28 bytes an element for fp32 parameters with 32-bit moments, 16 with 8-bit ones, 10 for bf16 parameters and
+// gradients with 8-bit moments; a wave has all loads of its 1024 elements in flight, and nothing moves twice.
+//
+// Measured (MI355X; a copy of 1 GiB runs at 5.3 TB/s on it), one tensor of 100 M elements: fp32 with 32 bits 522 us =
+// 5.4 TB/s, fp32 with 8 bits 299 us = 5.3, bf16 with 8 bits 194 us = 5.2 (where 47 vector instructions an element take
+// nearly as long as the memory); the 16 tensors of an h = 800 cell (2.6 M) 13.2 us, of an h = 200 cell 3.8 us.
 //
 // 8-bit moments.  256 elements (a wave's 64 lanes with 4 each: its maximum needs no LDS) share two powers of
 // two.  m is a sign, 4 exponent and 3 mantissa bits under 2^em, v 5 and 3 bits without a sign under 2^ev:
@@ -18,8 +23,8 @@
 //
 // The cut is random: 20 hashed bits (12 for m) are added below the code's last bit.  A step changes v by
 // (1 - b2) of itself, 0.1 % at b2 = 0.999, against half a code's 6 %: rounding to nearest would leave v where it
-// is for good, rounding at random keeps its mean.  The same holds for bf16 parameters (half a step is 2^-9 of
-// the value, lr is 1e-4).  A v that is not zero does not become zero: m / sqrt(v) would jump.
+// is for good, rounding at random keeps its mean.  The same holds for bf16 parameters (half a step is 2^-9
+// to 2^-8 of the value, lr is 1e-4).  A v that is not zero does not become zero: m / sqrt(v) would jump.
 // The 32 bits belong to (seed, step, the tensor's place, the element's place), so a run can be repeated.
 #include <string.h>
 
@@ -448,7 +453,8 @@ __global__ void adam_place_kernel(const AdamPlace a) {
   a.to[k] = d;
 }
 
-// The codes' values, 1024 per wave.
+// The codes' values, 1024 per wave.  HBM: 2 bytes in and 4 (bf16) out an element; 100 M of them 98 us = 6.1 TB/s, partly
+// from the last-level cache that the step left them in.
 template <typename T, int QUADS, bool FULL> IADMM_DEV void decode_wave(int64_t n, const uint8_t* m8, const uint8_t* v8,
                                                                        const int8_t* e, T* m, T* v, int64_t at) {
   const int lane = threadIdx.x % kWave;
@@ -487,6 +493,8 @@ template <typename T> __global__ void __launch_bounds__(256) adam_decode_kernel(
 }
 
 // ---------------------------------------------------------------------------------------------- the norm
+// sqrt(sum g^2), HBM bound: each workgroup sums a run of neighbouring chunks, one more the workgroups' sums.
+// 100 M bf16 elements in 216 tensors 41 us = 4.9 TB/s, 2.6 M fp32 ones 8 us (two launches).
 struct NormTensor {
   const void* g;
   int64_t n;

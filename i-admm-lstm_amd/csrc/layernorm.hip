@@ -10,6 +10,11 @@
 // Bound: HBM.  Forward 2 e bytes an element, backward 3 e (e = element size), ~8 and ~14 flop an element.  So
 // a row is read once and stays in registers, as the 16-byte vectors that it came in: TPR threads hold it (16,
 // 64, 256 or 1024; row_threads_fwd / row_threads_bwd), longer rows are read again, from L2 for the most part.
+//
+// Measured (MI355X; a copy of 1 GiB runs at 5.3 TB/s on it): forward 256000 x 800 fp32 281 us = 5.8 TB/s,
+// 8192 x 4096 bf16 26 us, 4000 x 800 fp32 6.5 us, one row 2.3 us; backward 470 us = 5.2 TB/s, 43 us = 4.7, 16 us.
+// Rows of 1025 to 4096 elements of 16 bits are the backward's weakest (four waves to a row, which wait for each
+// other): 20000 x 2500 bf16 84 us = 3.6 TB/s.
 #include <type_traits>
 
 #include "common.h"
@@ -157,6 +162,7 @@ struct LnFwd {
   int w32;
 };
 
+// Forward.  Bound by HBM from some thousand rows on, by the launch and one trip to memory and back below.
 // One row per TPR threads, NV vectors each; SHORT: rows shorter than a vector (TPR = 16, NV = 1).
 template <typename T, int TPR, int NV, bool SHORT>
 __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) ln_fwd_kernel(LnFwd a) {
@@ -401,7 +407,8 @@ template <typename T, int TPR, int NV, int BLOCK, bool SHORT> __global__ void __
   }
 }
 
-// Long rows: dx from two readings of the row, dw and db by columns (ln_bwd_cols_kernel).
+// Long rows: dx from two readings of the row (the second from the L2), dw and db by columns (ln_bwd_cols_kernel), a
+// third: HBM bound, 5 e bytes an element for 3 e.
 template <typename T> __global__ void __launch_bounds__(1024) ln_bwd_long_kernel(LnBwd a) {
   constexpr int V = Pack<T>::n, TPR = 1024;
   __shared__ float red[2][2 * TPR / kWave];
@@ -466,7 +473,7 @@ template <typename T> __global__ void __launch_bounds__(256) ln_bwd_cols_kernel(
 }
 
 // dw, db = the slabs' sums, in 64 bits: 64 columns x 16 runs of slabs per workgroup, so that a thread has 16
-// loads at most to wait for, and the runs meet in LDS in their order.
+// or 32 loads to wait for, and the runs meet in LDS in their order.  2 to 5 us (512 slabs of 4096 columns, 16.8 MB).
 template <typename W> __global__ void __launch_bounds__(1024) ln_slab_kernel(const float* slab, int slabs, int64_t cols,
                                                                             W* dw, W* db) {
   __shared__ double part[16][64];
