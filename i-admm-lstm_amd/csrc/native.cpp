@@ -49,6 +49,13 @@ int type_code(at::ScalarType t) {
 void on_device(const Tensor& t, const char* what, const Tensor* like = nullptr) {
   TORCH_CHECK_VALUE(t.is_cuda(), "iadmm kernels need device tensors (no CPU fallback), and ", what, " is on ", t.device());
   TORCH_CHECK_VALUE(!like || t.device() == like->device(), what, " is on ", t.device(), ", not on ", like->device());
+  TORCH_CHECK_VALUE(!t.is_neg(), what, " is a view that torch negates on reading: resolve_neg() it first");
+}
+
+// A kernel wrote it behind autograd's back: whoever goes by its version (a graph that saved it, solver.PackedWeights) has
+// to see it.
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
 Tensor f32_on(const Tensor& like, at::IntArrayRef shape) { return at::empty(shape, like.options().dtype(at::kFloat)); }
@@ -199,11 +206,11 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 
 // -------------------------------------------------------------------------------------- the optimizer's step
 struct List {
-  std::vector<Tensor> t;  // undefined where None
+  std::vector<Tensor> t;
   c10::Device device{at::kCPU};
 };
 
-// The items that `use` names (all where it is null), contiguous, on one device and of the given types.
+// The items that `use` names, contiguous, on one device and of the given types.
 List list_of(PyObject* seq, const char* what, std::initializer_list<at::ScalarType> types, const std::vector<int>& use) {
   List l;
   l.t.reserve(use.size());
@@ -215,7 +222,7 @@ List list_of(PyObject* seq, const char* what, std::initializer_list<at::ScalarTy
     TORCH_CHECK_TYPE(std::find(types.begin(), types.end(), t.scalar_type()) != types.end(), what, " must be ",
                      *types.begin(), types.size() > 1 ? " or " : "", types.size() > 1 ? toString(*(types.end() - 1)) : "",
                      ", got ", t.scalar_type());
-    TORCH_CHECK_VALUE(t.layout() == at::kStrided && t.is_contiguous(), what, " must be contiguous");
+    TORCH_CHECK_VALUE(t.layout() == at::kStrided && t.is_contiguous() && !t.is_neg(), what, " must be contiguous");
     TORCH_CHECK_VALUE(t.is_cuda(), "iadmm kernels need device tensors (no CPU fallback), and one of ", what, " is on ",
                       t.device());
     TORCH_CHECK_VALUE(l.t.size() == 1 || t.device() == l.device, what, " must be on one device, got ", t.device(), " and ",
@@ -289,12 +296,13 @@ PyObject* py_layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const at::AutoGradMode off(false);
   Tensor t[3];
   t[0] = ln_forward(x, w, b, eps, optional_tensor(a[4], "out"), stats ? &t[1] : nullptr, stats ? &t[2] : nullptr);
+  if (a[4] != Py_None) written(t[0]);
   if (stats) return tuple_of(t, 3);
   return wrap(t[0]);
   END_HANDLE_TH_ERRORS
 }
 
-// layer_norm_bwd(dy, x, mean, rstd, weight, wdtype_like, need_x, need_w, need_b); wdtype_like: a tensor or None
+// layer_norm_bwd(dy, x, mean, rstd, weight, type code without a weight, need_x, need_w, need_b)
 PyObject* py_layer_norm_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   want(n, 9);
@@ -435,9 +443,8 @@ PyObject* py_adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
        abi.adamw_step(many, rec.data(), eight ? 8 : 32, lr, lr_dev.defined() ? lr_dev.const_data_ptr<float>() : nullptr, b1, b2,
                       eps, decay, norm.defined() ? norm.const_data_ptr<float>() : nullptr, most, seed,
                       counted ? counts.mutable_data_ptr<int64_t>() : nullptr, address_of(ws), bytes, stream_of(p.device)));
-  // the kernel wrote behind autograd's back: whoever goes by the version (solver.PackedWeights) has to see it
-  for (const Tensor& t : p.t)
-    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+  for (const List* l : {&p, &m, &v})
+    for (const Tensor& t : l->t) written(t);
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }

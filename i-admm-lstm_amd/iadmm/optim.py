@@ -49,6 +49,8 @@ class AdamW(torch.optim.Optimizer):
         for p in self.param_groups[-1]["params"]:
             if p.dtype not in (torch.float32, torch.bfloat16):
                 raise TypeError(f"parameters must be float32 or bfloat16, got {p.dtype}")
+            if not p.is_contiguous():
+                raise ValueError(f"parameters must be contiguous, got strides {p.stride()} for {tuple(p.shape)}")
 
     def _state(self, p):
         """The state of one parameter, zeros at first."""
@@ -124,6 +126,8 @@ class AdamW(torch.optim.Optimizer):
         state with 32 bits does not load into 8; one with 8 bits loads into 32."""
         of = [(p, state_dict["state"].get(i)) for group, saved in zip(self.param_groups, state_dict["param_groups"])
               for p, i in zip(group["params"], saved["params"])]
+        if any(g.get("maximize") or g.get("amsgrad") for g in state_dict["param_groups"]):
+            raise ValueError("a state of an optimizer with maximize or amsgrad does not load")
         for p, s in of:
             if s is None or not s:
                 continue

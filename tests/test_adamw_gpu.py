@@ -525,6 +525,10 @@ def test_numbers_of_numpy():
     assert torch.equal(A[0][0], C[0][0])
     with pytest.raises((TypeError, ValueError)):
         ops.adamw_step(*A[:4], 3.5)
+    neg = torch._neg_view(A[1][0])
+    for call in (lambda: ops.adamw_step(A[0], [neg], A[2], A[3], 4), lambda: ops.grad_norm([neg])):
+        with pytest.raises(ValueError):
+            call()
 
 
 def test_a_step_is_seen_by_the_version():

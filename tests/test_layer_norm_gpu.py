@@ -252,6 +252,54 @@ def test_frozen_parts_get_no_gradient():
         assert not autograd.layer_norm(x, w, b).requires_grad
 
 
+def test_writing_into_a_saved_tensor_is_noticed():
+    """An out that a graph has saved: its backward refuses, as with torch's own in-place operations."""
+    from iadmm import autograd, ops
+    x, dy, w, b = inputs(5, 64, F32, F32)
+    w.requires_grad_(True)
+    y = autograd.layer_norm(x, w, b)
+    ops.layer_norm(x, out=x)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward(dy)
+
+
+def test_gradients_without_rows():
+    from iadmm import autograd
+    x, w = torch.zeros(0, 3, 40, device="cuda", requires_grad=True), torch.ones(40, device="cuda", requires_grad=True)
+    dx, dw = torch.autograd.grad(autograd.layer_norm(x, w).sum(), (x, w))
+    assert dx.shape == x.shape and bool((dw == 0).all())
+
+
+def test_two_threads_on_two_streams():
+    """Forward and gradients from two Python threads at once, each on its own stream: the bits of one after the other."""
+    import threading
+    from iadmm import autograd
+    cases = [inputs(2000, 800, F32, F32, seed=s) for s in (1, 2)]
+
+    def run(c):
+        x, w, b = (t.detach().clone().requires_grad_(True) for t in (c[0], c[2], c[3]))
+        y = autograd.layer_norm(x, w, b)
+        return (y.detach(), *torch.autograd.grad(y, (x, w, b), c[1]))
+
+    want = [run(c) for c in cases]
+    torch.cuda.synchronize()
+    got = [None, None]
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got[i] = run(cases[i])
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for a, c in zip(want, got):
+        assert all(torch.equal(p, q) for p, q in zip(a, c))
+
+
 def test_gradient_of_the_gradient_is_refused():
     from iadmm import autograd
     x, dy, w, b = inputs(4, 50, F32, F32)

@@ -107,6 +107,8 @@ def test_optimizer_arguments():
             AdamW(p, **kw)
     with pytest.raises(TypeError):
         AdamW([torch.nn.Parameter(torch.zeros(3, dtype=torch.float16))])
+    with pytest.raises(ValueError, match="contiguous"):
+        AdamW([torch.nn.Parameter(torch.zeros(3, 4).t())])
     opt = AdamW(p)
     assert opt.step() is None and not opt.state  # no gradient: nothing to do
     p[0].grad = torch.ones(3)

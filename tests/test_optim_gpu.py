@@ -108,6 +108,10 @@ def test_states_of_other_optimizers():
     for p, q in zip(eight.param_groups[0]["params"], wide.param_groups[0]["params"]):
         for x, y in zip(eight.moments(p), wide.moments(q)):
             assert torch.equal(x, y) and x.dtype == torch.float32
+    with pytest.raises(ValueError, match="maximize"):
+        up = torch.optim.AdamW(a, maximize=True)
+        up.step()
+        opt.load_state_dict(up.state_dict())
     with pytest.raises(ValueError, match="amsgrad"):
         ams = torch.optim.Adam(a, amsgrad=True)
         ams.step()
