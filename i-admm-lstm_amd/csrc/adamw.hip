@@ -570,6 +570,9 @@ __global__ void __launch_bounds__(1024) norm_end_kernel(const double* part, int 
 // Workgroups take 2048 elements at a time up to this many in all, 8192 above: 168 000 of them 7.1 us against 7.7 (with the
 // last sum's launch), 2.6 M 8.2 against 8.0.
 constexpr int64_t kNormSmall = int64_t{1} << 19;
+// Chunks of 1024 that one workgroup sums alone (16 waves, two rounds): 16 tensors of 2000 elements 5.8 us a call, 8.3 with
+// two launches; with four rounds the GPU takes 7.2 us, the two launches' 5.5.
+constexpr int64_t kNormFew = 32;
 template <int QUADS> static int launch_norm(NormLaunch& a, hipStream_t st) {  // gives its workgroups
   uint64_t chunks = 0;
   for (int k = 0; k < a.count; ++k) {
@@ -585,6 +588,35 @@ template <int QUADS> static int launch_norm(NormLaunch& a, hipStream_t st) {  //
 // Workgroups of 1024 elements up to this many in all, of 4096 above: 168 000 of them 7.9 us against 8.9 (with the
 // counting launch), 2.6 M 17.9 against 16.6.
 constexpr int64_t kAdamSmall = int64_t{1} << 19;
+// Few elements: one workgroup and one launch, 1024 elements to a wave at a time.
+struct NormFew {
+  NormLaunch a;
+  float* norm;
+};
+__global__ void __launch_bounds__(1024) norm_few_kernel(const NormFew f) {
+  __shared__ double red[16];
+  const int lane = threadIdx.x % kWave;
+  double s = 0.0;
+  for (uint32_t c = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave); c < f.a.chunks; c += 16) {
+    const NormTensor& t = f.a.t[find_tensor(f.a.t, f.a.count, c)];
+    const int64_t at = static_cast<int64_t>(c - t.first) * 1024;
+    for (int u = 0; u < 4; ++u) {
+      const int64_t i = at + u * 256 + lane * 4;
+      if (t.half) {
+        const Quad<__bf16> q = load_quad(static_cast<const __bf16*>(t.g) + i, t.n - i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s = fma(static_cast<float>(q.v[j]), static_cast<double>(static_cast<float>(q.v[j])), s);
+      } else {
+        const Quad<float> q = load_quad(static_cast<const float*>(t.g) + i, t.n - i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s = fma(static_cast<double>(q.v[j]), static_cast<double>(q.v[j]), s);
+      }
+    }
+  }
+  s = block_sum_f64(s, red);
+  if (threadIdx.x == 0) *f.norm = static_cast<float>(sqrt(s));
+}
+
 template <bool EIGHT, int QUADS> static void launch_adam(const AdamLaunch& a, const AdamTensor* table, unsigned blocks,
                                                        hipStream_t st) {
   if (table)
@@ -617,7 +649,20 @@ extern "C" int iadmm_grad_norm(int64_t count, const iadmm_grad_tensor* grads, fl
   int parts = 0;
   NormLaunch a;
   a.count = 0;
-  int64_t total = 0;
+  int64_t total = 0, few = 0;
+  for (int64_t i = 0; i < count; ++i) few += (grads[i].n + 1023) / 1024;
+  if (count <= kNormPer && few <= kNormFew) {
+    NormFew f;
+    f.norm = norm, f.a.count = 0, f.a.part = nullptr, f.a.chunks = static_cast<uint32_t>(few);
+    uint32_t first = 0;
+    for (int64_t i = 0; i < count; ++i) {
+      f.a.t[f.a.count++] = NormTensor{grads[i].g, grads[i].n, first, grads[i].dtype == IADMM_BF16};
+      first += static_cast<uint32_t>((grads[i].n + 1023) / 1024);
+    }
+    hipLaunchKernelGGL(norm_few_kernel, dim3(1), dim3(1024), 0, st, f);
+    IADMM_CHECK_LAUNCH();
+    return IADMM_OK;
+  }
   for (int64_t i = 0; i < count; ++i) {
     if (grads[i].n > 0) {
       a.t[a.count++] = NormTensor{grads[i].g, grads[i].n, 0u, grads[i].dtype == IADMM_BF16};

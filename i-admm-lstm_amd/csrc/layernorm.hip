@@ -276,6 +276,7 @@ struct LnBwd {
   void* dx;     // or null
   float* slab;  // [gridDim.x][2][cols]: each workgroup's share of dw and db; or null
   int w32;
+  void *dw, *db;  // of a workgroup that has all rows: it writes them itself; or null
 };
 
 // A workgroup of BLOCK threads takes BLOCK / TPR rows at a time, one workgroup per CU at most: dw and db grow in
@@ -363,7 +364,7 @@ template <typename T, int TPR, int NV, int BLOCK, bool SHORT> __global__ void __
       }
     }
   }
-  if (!a.slab) return;
+  if (!a.slab && !a.dw && !a.db) return;
   // The groups' sums meet in LDS: first those of a wave's own groups by shuffles, then all at once, and each column
   // adds the groups in their order.  (One group after the other took 16 us for the 16 of 800 columns.)
   constexpr int SHARE = TPR < kWave ? kWave / TPR : 1, PITCH = TPR * E;
@@ -402,7 +403,10 @@ template <typename T, int TPR, int NV, int BLOCK, bool SHORT> __global__ void __
       float s = lds[c];
 #pragma unroll
       for (int g = 1; g < R / SHARE; ++g) s += lds[g * PITCH + c];
-      out[half * cols + c] = s;
+      void* whole = half ? a.db : a.dw;
+      if (a.slab) out[half * cols + c] = s;
+      else if (whole && (sizeof(T) == 4 || a.w32)) static_cast<float*>(whole)[c] = s;
+      else if (whole) static_cast<T*>(whole)[c] = static_cast<T>(s);
     }
   }
 }
@@ -512,8 +516,16 @@ static int bwd_block(int64_t cols, int tpr) { return tpr == 256 || (tpr == 64 &&
 // while the other waits.
 static int64_t bwd_most(int tpr) { return tpr == 256 ? 2 * kCUs : kCUs; }
 
+// One workgroup alone, without slabs and their sum: one round of rows, or two of the shortest (128 rows of 40 fp32: 6.1 us
+// a call, 129 with slabs 9.6; a second round of 16 rows of 800 takes the GPU 9.3 us, slabs 8.4).
+static bool bwd_alone(int64_t rows, int64_t cols, int vec) {
+  if (cols > kMaxHeld) return false;
+  const int tpr = row_threads_bwd(cols, vec);
+  return rows <= bwd_block(cols, tpr) / tpr * (tpr == 16 ? 2 : 1);
+}
+
 static int64_t bwd_slabs(int64_t rows, int64_t cols, int vec) {
-  if (rows <= 0) return 0;
+  if (rows <= 0 || bwd_alone(rows, cols, vec)) return 0;
   if (cols > kMaxHeld) {  // column kernel: enough row runs for ~4 workgroups per CU
     const int64_t blocks = (cols + 256 * vec - 1) / (256 * vec);
     const int64_t runs = (4 * kCUs + blocks - 1) / blocks;
@@ -628,19 +640,22 @@ extern "C" int iadmm_layer_norm_bwd(int64_t rows, int64_t cols, int dtype, int w
   const bool sums = dw || db;
   if (rows > 0 && (!dy || !x || !mean || !rstd || lddy < cols || ldx < cols)) return IADMM_E_ARG;
   if (sums && ws_bytes < iadmm_layer_norm_bwd_ws_bytes(rows, cols, dtype)) return IADMM_E_ARG;
-  if (sums && rows > 0 && !ws) return IADMM_E_ARG;
+  if (sums && rows > 0 && !ws && iadmm_layer_norm_bwd_ws_bytes(rows, cols, dtype) > 0) return IADMM_E_ARG;
   if (sums && !aligned16(ws)) return IADMM_E_ALIGN;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const int64_t slabs = bwd_slabs(rows, cols, dtype == IADMM_F32 ? 4 : 8);
-  const LnBwd a{rows, cols, lddy, ldx, dy, x, w, mean, rstd, dx, sums ? static_cast<float*>(ws) : nullptr,
-                wdtype == IADMM_F32};
+  const int vec = dtype == IADMM_F32 ? 4 : 8;
+  const bool alone = rows > 0 && bwd_alone(rows, cols, vec);
+  const int64_t slabs = bwd_slabs(rows, cols, vec), most = bwd_most(row_threads_bwd(cols, vec));
+  const LnBwd a{rows, cols, lddy, ldx, dy, x, w, mean, rstd, dx, sums && !alone ? static_cast<float*>(ws) : nullptr,
+                wdtype == IADMM_F32, alone ? dw : nullptr, alone ? db : nullptr};
   if (rows > 0 && (dx || sums)) {
-    const int rc = dtype == IADMM_F32 ? bwd<float>(a, slabs, st)
-                   : dtype == IADMM_BF16 ? bwd<__bf16>(a, slabs, st) : bwd<_Float16>(a, slabs, st);
+    const int64_t blocks = alone && sums ? 1 : alone ? (rows < most ? rows : most) : slabs;
+    const int rc = dtype == IADMM_F32 ? bwd<float>(a, blocks, st)
+                   : dtype == IADMM_BF16 ? bwd<__bf16>(a, blocks, st) : bwd<_Float16>(a, blocks, st);
     if (rc) return rc;
     IADMM_CHECK_LAUNCH();
   }
-  if (sums) {  // (no rows: the sums are 0)
+  if (sums && !alone) {  // (no rows: the sums are 0)
     const dim3 grid(static_cast<unsigned>((2 * cols + 63) / 64)), block(1024);
     const float* slab = static_cast<const float*>(ws);
     const int n = static_cast<int>(slabs);

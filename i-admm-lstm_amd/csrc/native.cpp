@@ -158,7 +158,7 @@ std::vector<Tensor> ln_backward(const Tensor& dy, const Tensor& x, const Tensor&
   int64_t bytes = 0;
   if (need_w || need_b) {
     bytes = abi.ln_bwd_ws_bytes(r.rows, r.cols, t);
-    ws = f32_on(x, {bytes / 4});
+    if (bytes) ws = f32_on(x, {bytes / 4});
   }
   const c10::DeviceGuard guard(x.device());
   done("iadmm_layer_norm_bwd",

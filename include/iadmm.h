@@ -368,7 +368,7 @@ int iadmm_loss_grad_split(int64_t B, int64_t n, int64_t m, const float* Q, const
  *     dx = rstd (q - mean(q) - xhat mean(q xhat)), q = dy w; dw = sum_rows dy xhat; db = sum_rows dy;
  *     each may be NULL.  The sums over rows have a fixed order (bitwise reproducible).  ws: caller-owned
  *     16-B aligned workspace of iadmm_layer_norm_bwd_ws_bytes(rows, cols, dtype) bytes (unused where dw
- *     and db are NULL).  rows = 0 writes dw = db = 0. */
+ *     and db are NULL, or where the size is 0).  rows = 0 writes dw = db = 0. */
 enum { IADMM_F32 = 0, IADMM_BF16 = 1, IADMM_F16 = 2 };
 int iadmm_layer_norm_fwd(int64_t rows, int64_t cols, int dtype, int wdtype, const void* x, int64_t ldx,
                          const void* w, const void* b, float eps, void* y, float* mean, float* rstd,

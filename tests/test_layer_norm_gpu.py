@@ -72,7 +72,7 @@ def close(got, want, tol, what):
     assert bool((over <= 0).all()), f"{what}: off by {float(off.max()):.3g}, {float(over.max()):.3g} more than allowed"
 
 
-SHAPES = [(1, 1), (3, 2), (5, 40), (7, 127), (1, 200), (9, 129), (4, 256), (130, 257), (65, 800), (6, 1000),
+SHAPES = [(16, 800), (17, 800), (32, 1000), (128, 40), (129, 40), (127, 3), (4, 2100), (1, 12000), (2, 12000), (1, 1), (3, 2), (5, 40), (7, 127), (1, 200), (9, 129), (4, 256), (130, 257), (65, 800), (6, 1000),
           (33, 1025), (300, 7), (1000, 64), (5, 2049), (9, 4097), (3, 9001), (3, 16384), (2, 16385), (5, 20003)]
 TYPES = [(F32, F32), (BF16, F32), (BF16, BF16), (F16, F32), (F16, F16)]
 
