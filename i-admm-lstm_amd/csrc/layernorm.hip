@@ -9,12 +9,12 @@
 //
 // Bound: HBM.  Forward 2 e bytes an element, backward 3 e (e = element size), ~8 and ~14 flop an element.  So
 // a row is read once and stays in registers, as the 16-byte vectors that it came in: TPR threads hold it (16,
-// 64, 256 or 1024; row_threads_fwd / row_threads_bwd), longer rows are read again, from L2 for the most part.
+// or 64 to 1024; row_threads_fwd / row_threads_bwd), longer rows are read again, from L2 for the most part.
 //
-// Measured (MI355X; a copy of 1 GiB runs at 5.3 TB/s on it): forward 256000 x 800 fp32 281 us = 5.8 TB/s,
-// 8192 x 4096 bf16 26 us, 4000 x 800 fp32 6.5 us, one row 2.3 us; backward 470 us = 5.2 TB/s, 43 us = 4.7, 16 us.
-// Rows of 1025 to 4096 elements of 16 bits are the backward's weakest (four waves to a row, which wait for each
-// other): 20000 x 2500 bf16 84 us = 3.6 TB/s.
+// Measured (MI355X; a copy of 1 GiB runs at 5.3 TB/s on it): forward 256000 x 800 fp32 284 us = 5.8 TB/s, 8192 x 4096
+// bf16 24, 4000 x 800 fp32 6, one row 1.8; backward of the first three 436 (5.6 TB/s), 41 and 12 us with the slabs' sum.
+// 100 M elements, 100 to 16384 columns: forward 4.2 to 5.2 TB/s in 16 bits, 5.0 to 5.7 in 32; backward 3.9 to 5.1 and
+// 4.7 to 5.5, lowest where a row fills its threads badly (513, 1200 columns).
 #include <type_traits>
 
 #include "common.h"
@@ -55,18 +55,22 @@ template <typename T> IADMM_DEV void set(Pack<T>& p, const float (&v)[Pack<T>::n
 // flight together (8192 rows of 4096 bf16: 48 us with branches, 26 without).  The elements that its neighbours
 // hold too are its first `dup`: they count in no sum, and their result is stored twice, with the same bits.
 struct Place {
-  int64_t at;  // column of its first element
+  uint32_t at;  // column of its first element
   int dup;
 };
-template <typename T> IADMM_DEV Place place(int64_t c, int64_t cols) {
+template <typename T> IADMM_DEV Place place(int c, int cols) {
   constexpr int V = Pack<T>::n;
-  const int64_t last = cols - V, at = c < last ? c : last;
-  return Place{at, static_cast<int>(c - at)};
+  const int last = cols - V, at = c < last ? c : last;
+  return Place{static_cast<uint32_t>(at), c - at};
 }
-template <typename T> IADMM_DEV Pack<T> load_whole(const T* p) {
+// 16 bytes from element `at` (32 bits of offset beside a base that a wave shares: no arithmetic in 64 bits per access).
+template <typename T> IADMM_DEV Pack<T> load_whole(const T* p, uint32_t at) {
   Pack<T> r;
-  __builtin_memcpy(&r, p, 16);
+  __builtin_memcpy(&r, reinterpret_cast<const char*>(p) + at * static_cast<uint32_t>(sizeof(T)), 16);
   return r;
+}
+template <typename T> IADMM_DEV void store_whole(T* p, uint32_t at, const Pack<T>& r) {
+  __builtin_memcpy(reinterpret_cast<char*>(p) + at * static_cast<uint32_t>(sizeof(T)), &r, 16);
 }
 
 // n elements from p; what lies behind is 0.  For rows shorter than a vector and for the long rows' kernels.
@@ -115,27 +119,51 @@ IADMM_DEV void load_weights(const void* w, bool f32, int64_t c, int64_t cols, fl
   } else if (sizeof(T) == 4 || f32) {
 #pragma unroll
     for (int k = 0; k < V / 4; ++k) {
-      const float* p = static_cast<const float*>(w) + c + 4 * k;
-      const Pack<float> a = WHOLE ? load_whole(p) : load_pack(p, n - 4 * k);
+      const float* p = static_cast<const float*>(w) + 4 * k;
+      const Pack<float> a = WHOLE ? load_whole(p, static_cast<uint32_t>(c)) : load_pack(p + c, n - 4 * k);
 #pragma unroll
       for (int j = 0; j < 4; ++j) out[4 * k + j] = get(a, j);
     }
   } else {
-    const T* p = static_cast<const T*>(w) + c;
-    const Pack<T> a = WHOLE ? load_whole(p) : load_pack(p, n);
+    const T* p = static_cast<const T*>(w);
+    const Pack<T> a = WHOLE ? load_whole(p, static_cast<uint32_t>(c)) : load_pack(p + c, n);
 #pragma unroll
     for (int j = 0; j < V; ++j) out[j] = get(a, j);
   }
 }
 
-// Sums of v over the TPR threads of a row, in every one of them.  More than a wave: through LDS, `red` holding
-// one value per wave of the workgroup; the caller alternates between two such arrays, so one barrier is enough
-// (a wave writes an array again only after every wave has passed the other array's barrier).
+// Sums of v over the TPR threads of a row, in every one of them.  Within 16 lanes and then a wave by adds whose second
+// operand comes from another lane, a few cycles each (through LDS a step waits for some hundred); over the waves
+// through LDS, `red` holding one value per wave of the workgroup; the caller alternates between two such arrays,
+// so one barrier is enough (a wave writes an array again only after every wave has passed the other array's barrier).
+template <int CTRL> IADMM_DEV float add_from(float v) {
+  return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, true));
+}
+template <int N> IADMM_DEV float sum_lanes(float v) {  // over N neighbours, up to 16, in each of them
+  if (N >= 2) v = add_from<0xB1>(v);    // within quads: 1 lane apart,
+  if (N >= 4) v = add_from<0x4E>(v);    // 2 lanes apart
+  if (N >= 8) v = add_from<0x141>(v);   // half rows mirrored
+  if (N >= 16) v = add_from<0x140>(v);  // rows mirrored
+  return v;
+}
+// Over lanes 16, 32 and 48 apart: halves, then rows of 16, change places between a register and its copy.
+IADMM_DEV float sum_rows16(float v) {
+  const uint32_t a = __float_as_uint(v);
+  const auto h = __builtin_amdgcn_permlane32_swap(a, a, false, false);
+  const uint32_t b = __float_as_uint(__uint_as_float(h[0]) + __uint_as_float(h[1]));
+  const auto q = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+  return __uint_as_float(q[0]) + __uint_as_float(q[1]);
+}
 template <int TPR, int K> IADMM_DEV void row_sum(float (&v)[K], float* red) {
+  static_assert(TPR == 16 || (TPR >= kWave && TPR <= 1024), "");
 #pragma unroll
-  for (int o = (TPR < kWave ? TPR : kWave) / 2; o >= 1; o >>= 1)
-#pragma unroll
-    for (int k = 0; k < K; ++k) v[k] += __shfl_xor(v[k], o, kWave);
+  for (int k = 0; k < K; ++k) {
+    v[k] = sum_lanes<16>(v[k]);
+    if constexpr (TPR >= kWave) {
+      v[k] = add_from<0x143>(add_from<0x142>(v[k]));  // row_bcast 15, 31: lane 63 has the wave's
+      v[k] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v[k]), 63));
+    }
+  }
   if constexpr (TPR > kWave) {
     constexpr int W = TPR / kWave;
     const int wave = threadIdx.x / kWave;
@@ -143,14 +171,17 @@ template <int TPR, int K> IADMM_DEV void row_sum(float (&v)[K], float* red) {
 #pragma unroll
       for (int k = 0; k < K; ++k) red[wave * K + k] = v[k];
     __syncthreads();
-    const float* r = red + wave / W * W * K;
+    const float* r = red + (wave / W * W + threadIdx.x % W) * K;
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      float s = r[k];
-      for (int w = 1; w < W; ++w) s += r[w * K + k];
-      v[k] = s;
-    }
+    for (int k = 0; k < K; ++k)
+      v[k] = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(sum_lanes<W>(r[k]))));
   }
+}
+
+// What the threads of a wave share: their row's number, and the first column of their vector i (TPR < 64: of all rows).
+template <int TPR> IADMM_DEV int shared(int v) { return TPR >= kWave ? __builtin_amdgcn_readfirstlane(v) : v; }
+template <typename T, int TPR> IADMM_DEV int first_col(int i) {
+  return (i * TPR + (TPR > kWave ? __builtin_amdgcn_readfirstlane(threadIdx.x % TPR) : 0)) * Pack<T>::n;
 }
 
 struct LnFwd {
@@ -168,35 +199,37 @@ template <typename T, int TPR, int NV, bool SHORT>
 __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) ln_fwd_kernel(LnFwd a) {
   constexpr int V = Pack<T>::n, BLOCK = TPR > 256 ? TPR : 256, R = BLOCK / TPR;
   __shared__ float red[2][BLOCK / kWave];
-  const int lane = threadIdx.x % TPR;
-  const float inv = 1.0f / static_cast<float>(a.cols);
+  const int lane = threadIdx.x % TPR, cols = static_cast<int>(a.cols);
+  const float inv = 1.0f / static_cast<float>(cols);
   // (no loop over rows: the weights would be loaded before it and stay in 2 registers an element)
-  const int64_t row = (static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x) * R + threadIdx.x / TPR;
+  const int64_t row = (static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x) * R + shared<TPR>(threadIdx.x / TPR);
   const bool on = row < a.rows;
   const T* x = static_cast<const T*>(a.x) + (on ? row : 0) * a.ldx;
   Pack<T> p[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int64_t c = static_cast<int64_t>(i * TPR + lane) * V;
-    p[i] = SHORT ? load_pack(x + c, a.cols - c) : load_whole(x + place<T>(c, a.cols).at);
+    const int c = (i * TPR + lane) * V;
+    p[i] = SHORT ? load_pack(x + c, cols - c) : load_whole(x, place<T>(c, cols).at);
   }
-  // whether element j of vector i counts; only the row's last vectors have to ask (the same for all threads)
+  // Vector by vector, so that a path has 8 + NV additions.  Whether element j of vector i counts only the row's last
+  // vectors ask.
   auto sum = [&](auto term) {
-    float s[1] = {0.0f};
+    float s = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int64_t c = static_cast<int64_t>(i * TPR + lane) * V;
-      if (static_cast<int64_t>(i + 1) * TPR * V > a.cols) {
-        const int64_t left = a.cols - c;
-        const int dup = SHORT ? 0 : place<T>(c, a.cols).dup;
+      const int c = (i * TPR + lane) * V;
+      float t = 0.0f;
+      if ((i + 1) * TPR * V <= cols) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) s[0] += j >= dup && j < (SHORT ? left : V) ? term(get(p[i], j)) : 0.0f;
+        for (int j = 0; j < V; ++j) t += term(get(p[i], j));
       } else {
+        const int dup = SHORT ? 0 : place<T>(c, cols).dup;
 #pragma unroll
-        for (int j = 0; j < V; ++j) s[0] += term(get(p[i], j));
+        for (int j = 0; j < V; ++j) t += j >= dup && j < (SHORT ? cols - c : V) ? term(get(p[i], j)) : 0.0f;
       }
+      s += t;
     }
-    return s[0];
+    return s;
   };
   float s[1] = {sum([](float v) { return v; })};
   row_sum<TPR, 1>(s, red[0]);
@@ -209,15 +242,16 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) ln_fwd_kernel(LnFwd a) 
   auto finish = [&](auto kind) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int64_t c = static_cast<int64_t>(i * TPR + lane) * V;
-      const int64_t at = SHORT ? c : place<T>(c, a.cols).at;
+      const int c = (i * TPR + lane) * V;
+      const uint32_t at = SHORT ? c : place<T>(c, cols).at;
       float w[V], b[V];
       load_weights<T, !SHORT, kind()>(a.w, a.w32, at, a.cols, 1.0f, w);
       load_weights<T, !SHORT, kind()>(a.b, a.w32, at, a.cols, 0.0f, b);
 #pragma unroll
       for (int j = 0; j < V; ++j) w[j] = fmaf((get(p[i], j) - mu) * r, w[j], b[j]);
       set(p[i], w);
-      if (c < a.cols) store_pack(y + at, p[i], SHORT ? a.cols - at : V);
+      if (SHORT) store_pack(y + at, p[i], cols - c);
+      else if (c < cols) store_whole(y, at, p[i]);
     }
   };
   if (!a.w || !a.b || SHORT) finish(std::integral_constant<int, kAnyKind>());
@@ -279,19 +313,30 @@ struct LnBwd {
   void *dw, *db;  // of a workgroup that has all rows: it writes them itself; or null
 };
 
-// A workgroup of BLOCK threads takes BLOCK / TPR rows at a time, one workgroup per CU at most: dw and db grow in
+// A workgroup of BLOCK threads takes BLOCK / TPR rows at a time, 1024 threads per CU at most: dw and db grow in
 // registers over all its rows, meet once in LDS and leave as one slab, which keeps the slabs' traffic small beside
-// the rows' (256 slabs at most).  Up to 64 threads a row there is no barrier among them, and a wave waits for its
+// the rows' (512 slabs at most).  Up to 64 threads a row there is no barrier among them, and a wave waits for its
 // own rows alone.
 template <typename T, int TPR, int NV, int BLOCK, bool SHORT> __global__ void __launch_bounds__(BLOCK) ln_bwd_kernel(LnBwd a) {
-  constexpr int V = Pack<T>::n, R = BLOCK / TPR, E = NV * V;
+  constexpr int V = Pack<T>::n, R = BLOCK / TPR, E = NV * V, SPAN = (TPR < kWave ? TPR : kWave) * V;
   extern __shared__ float lds[];  // [groups][TPR * E]
   __shared__ float red[2][2 * BLOCK / kWave];
-  const int lane = threadIdx.x % TPR, group = threadIdx.x / TPR;
-  const float inv = 1.0f / static_cast<float>(a.cols);
-  float dw[E], db[E];
+  const int lane = threadIdx.x % TPR, group = shared<TPR>(threadIdx.x / TPR), cols = static_cast<int>(a.cols);
+  const float inv = 1.0f / static_cast<float>(cols);
+  // The weights stay in registers (read again for each row and pass, a wave waits for them four times: 24414 x 4096
+  // bf16 136 us, kept 118); at 24 elements a thread they would take those of four waves.
+  constexpr bool KEEP = E <= 16;
+  float dw[E], db[E], w[KEEP ? NV : 1][V];
 #pragma unroll
   for (int i = 0; i < E; ++i) dw[i] = db[i] = 0.0f;
+  uint32_t again = 0;
+  auto weights = [&](int i, float (&to)[V]) {
+    const int c = (i * TPR + lane) * V;
+    load_weights<T, !SHORT>(a.w, a.w32, (SHORT ? c : place<T>(c, cols).at) + again, cols, 1.0f, to);
+  };
+  if constexpr (KEEP)
+#pragma unroll
+    for (int i = 0; i < NV; ++i) weights(i, w[i]);
   int odd = 0;
   for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * R; row0 < a.rows;
        row0 += static_cast<int64_t>(gridDim.x) * R, odd ^= 1) {
@@ -300,67 +345,67 @@ template <typename T, int TPR, int NV, int BLOCK, bool SHORT> __global__ void __
     const int64_t from = on ? row : 0;
     const T* x = static_cast<const T*>(a.x) + from * a.ldx;
     const T* dy = static_cast<const T*>(a.dy) + from * a.lddy;
-    const void* weights = a.w;
-    asm volatile("" : "+s"(weights));  // read again for every row, from the L1: they would not fit the registers
     Pack<T> px[NV], pd[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int64_t c = static_cast<int64_t>(i * TPR + lane) * V;
+      const int c = (i * TPR + lane) * V;
       if constexpr (SHORT) {
-        px[i] = load_pack(x + c, a.cols - c);
-        pd[i] = load_pack(dy + c, a.cols - c);
+        px[i] = load_pack(x + c, cols - c);
+        pd[i] = load_pack(dy + c, cols - c);
       } else {
-        const int64_t at = place<T>(c, a.cols).at;
-        px[i] = load_whole(x + at);
-        pd[i] = load_whole(dy + at);
+        const uint32_t at = place<T>(c, cols).at;
+        px[i] = load_whole(x, at);
+        pd[i] = load_whole(dy, at);
       }
     }
     const float mu = a.mean[from], r = a.rstd[from];
     float s[2] = {0.0f, 0.0f};
     // xh and q are made twice from the row's 16-byte packs: as fp32 they would take twice to four times the registers
+    if (on) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int64_t c = static_cast<int64_t>(i * TPR + lane) * V;
-      const Place to = SHORT ? Place{c, 0} : place<T>(c, a.cols);
-      float w[V];
-      load_weights<T, !SHORT>(weights, a.w32, to.at, a.cols, 1.0f, w);
-      auto add = [&](int j) {
-        const float d = get(pd[i], j), h = (get(px[i], j) - mu) * r, q = d * w[j];
-        s[0] += q;
-        s[1] = fmaf(q, h, s[1]);
-        dw[i * V + j] = fmaf(d, h, dw[i * V + j]);
-        db[i * V + j] += d;
-      };
-      if (static_cast<int64_t>(i + 1) * TPR * V > a.cols || row0 + R > a.rows) {  // (the same for the workgroup)
-        const int64_t left = SHORT ? a.cols - c : V;
+      for (int i = 0; i < NV; ++i) {
+        const int c = (i * TPR + lane) * V, first = first_col<T, TPR>(i);
+        if (first >= cols) continue;
+        if constexpr (!KEEP) weights(i, w[0]);
+        const float (&wi)[V] = w[KEEP ? i : 0];
+        const Place to = SHORT ? Place{static_cast<uint32_t>(c), 0} : place<T>(c, cols);
+        auto add = [&](int j, bool own) {
+          const float d = get(pd[i], j), h = (get(px[i], j) - mu) * r, q = d * wi[j];
+          s[0] = own ? s[0] + q : s[0];
+          s[1] = own ? fmaf(q, h, s[1]) : s[1];
+          dw[i * V + j] = fmaf(d, h, dw[i * V + j]);  // (what is not its own it leaves behind below)
+          db[i * V + j] += d;
+        };
+        if (first + SPAN > cols) {  // only the wave that holds the row's end has to ask
+          const int left = SHORT ? cols - c : V;
 #pragma unroll
-        for (int j = 0; j < V; ++j)
-          if (on && j >= to.dup && j < left) add(j);
-      } else {
+          for (int j = 0; j < V; ++j) add(j, j >= to.dup && j < left);
+        } else {
 #pragma unroll
-        for (int j = 0; j < V; ++j) add(j);
+          for (int j = 0; j < V; ++j) add(j, true);
+        }
       }
     }
     row_sum<TPR, 2>(s, red[odd]);
+    if constexpr (!KEEP) asm volatile("" : "+s"(again));  // (0: so that they are not kept after all)
     if (a.dx && on) {
       const float s0 = s[0] * inv, s1 = s[1] * inv;
       T* dx = static_cast<T*>(a.dx) + row * a.cols;
-      asm volatile("" : "+s"(weights));
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int64_t c = static_cast<int64_t>(i * TPR + lane) * V;
-        if (c >= a.cols) continue;
-        const int64_t at = SHORT ? c : place<T>(c, a.cols).at;
-        float w[V];
-        load_weights<T, !SHORT>(weights, a.w32, at, a.cols, 1.0f, w);
+        const int c = (i * TPR + lane) * V;
+        if (c >= cols) continue;
+        const uint32_t at = SHORT ? c : place<T>(c, cols).at;
+        if constexpr (!KEEP) weights(i, w[0]);
+        const float (&wi)[V] = w[KEEP ? i : 0];
+        float v[V];
         Pack<T> p;
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float q = get(pd[i], j) * w[j], h = (get(px[i], j) - mu) * r;
-          w[j] = r * (q - fmaf(h, s1, s0));
-        }
-        set(p, w);
-        store_pack(dx + at, p, SHORT ? a.cols - at : V);
+        for (int j = 0; j < V; ++j)
+          v[j] = r * fmaf(-((get(px[i], j) - mu) * r), s1, fmaf(get(pd[i], j), wi[j], -s0));
+        set(p, v);
+        if (SHORT) store_pack(dx + at, p, cols - c);
+        else store_whole(dx, at, p);
       }
     }
   }
@@ -368,14 +413,9 @@ template <typename T, int TPR, int NV, int BLOCK, bool SHORT> __global__ void __
   // The groups' sums meet in LDS: first those of a wave's own groups by shuffles, then all at once, and each column
   // adds the groups in their order.  (One group after the other took 16 us for the 16 of 800 columns.)
   constexpr int SHARE = TPR < kWave ? kWave / TPR : 1, PITCH = TPR * E;
+  if constexpr (TPR < kWave)
 #pragma unroll
-  for (int o = kWave / 2; o >= TPR; o >>= 1)
-#pragma unroll
-    for (int i = 0; i < E; ++i) {
-      dw[i] += __shfl_xor(dw[i], o, kWave);
-      db[i] += __shfl_xor(db[i], o, kWave);
-    }
-  const int cols = static_cast<int>(a.cols);
+    for (int i = 0; i < E; ++i) dw[i] = sum_rows16(dw[i]), db[i] = sum_rows16(db[i]);
   float* out = a.slab + static_cast<int64_t>(blockIdx.x) * 2 * a.cols;
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
@@ -391,10 +431,10 @@ template <typename T, int TPR, int NV, int BLOCK, bool SHORT> __global__ void __
           for (int j = 0; j < V; j += 4)
             *reinterpret_cast<float4*>(to + c + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
         } else if (c < cols) {  // the last vector's own elements
-          const Place p = SHORT ? Place{c, 0} : place<T>(c, cols);
+          const Place p = SHORT ? Place{static_cast<uint32_t>(c), 0} : place<T>(c, cols);
 #pragma unroll
           for (int j = 0; j < V; ++j)
-            if (j >= p.dup && p.at + j < cols) to[p.at + j] = v[j];
+            if (j >= p.dup && static_cast<int>(p.at) + j < cols) to[p.at + j] = v[j];
         }
       }
     }
@@ -500,28 +540,35 @@ constexpr int kCUs = 256;
 constexpr int64_t kMaxCols = 1 << 24;  // (ln_slab_kernel's grid has 32 threads a column, of 2^32)
 constexpr int64_t kMaxHeld = 16384;  // elements of a row that a workgroup of the backward kernel holds
 
-// Threads per row, forward: as few as hold it with 8 vectors each, since fewer meet without a barrier (8192 rows
-// of 4096 bf16 took 42 us with 256 threads a row, 26 with 64).
+// Forward: threads per row.  Fewer take their sums with less waiting, but each has more to load: up to 3 vectors each
+// in a wave, 4 beyond (1500 columns of fp32: 64 threads 159 us for 400 MB, 128 147, 256 147 with half of them idle; 1200:
+// 150, 145, 149).  16 threads, whose sums stay among neighbours, with rows of 16 bits up to 5 vectors each (513 columns:
+// 98 us for 200 MB, 64 threads 141; 800 columns: 86 and 82), of 32 bits up to 2 (400 columns: 163 and 139).
 static int row_threads_fwd(int64_t cols, int vec) {
-  return cols <= 16 * 2 * vec ? 16 : cols <= 64 * 8 * vec ? 64 : cols <= 256 * 8 * vec ? 256 : 1024;
+  const int64_t n = (cols + vec - 1) / vec;
+  if (n <= 16 * (vec == 8 ? 5 : 2)) return 16;
+  return n <= 64 * 3 ? 64 : n <= 128 * 4 ? 128 : n <= 256 * 4 ? 256 : n <= 512 * 4 ? 512 : 1024;
 }
-// Backward: 16 elements each, beside which the sums of dw and db have room in 128 registers (1024 threads), or 32
-// in 256 (512 threads; 64 would spill).
+// Backward: up to 2 vectors each (3 in a wave, 4 where there are no more threads), beside which the weights and the sums
+// of dw and db leave registers for 16 waves a CU.  600 MB of 16 bits: 1200 columns take 142 us with 64 threads and 3
+// vectors, 155 with 128 and 2; 5000 columns 171 with 256 and 3 (12 waves), 131 with 512 and 2.
 static int row_threads_bwd(int64_t cols, int vec) {
-  if (cols <= 16 * 16) return vec == 8 || cols <= 16 * 8 ? 16 : 64;
-  return cols <= 64 * 32 ? 64 : cols <= 256 * 16 ? 256 : 1024;
+  const int64_t n = (cols + vec - 1) / vec;
+  if (n <= 16 * 2) return 16;
+  return n <= 64 * 3 ? 64 : n <= 128 * 2 ? 128 : n <= 256 * 2 ? 256 : n <= 512 * 2 ? 512 : 1024;
 }
-static int bwd_block(int64_t cols, int tpr) { return tpr == 256 || (tpr == 64 && cols > 64 * 16) ? 512 : 1024; }
-// Workgroups, and so slabs: one per CU; two where they are of 512 threads that meet at barriers, so that one loads
-// while the other waits.
-static int64_t bwd_most(int tpr) { return tpr == 256 ? 2 * kCUs : kCUs; }
+// Workgroups of 512 threads, two per CU, so that one loads while the other waits, where that tells (256 threads a row:
+// 2500 columns 128 us, 157 with 1024); elsewhere of 1024, which halves the slabs.
+static int bwd_block(int64_t cols, int tpr, int vec) {
+  return tpr == 256 || (tpr == 64 && cols > 64 * vec) ? 512 : 1024;
+}
 
-// One workgroup alone, without slabs and their sum: one round of rows, or two of the shortest (128 rows of 40 fp32: 6.1 us
-// a call, 129 with slabs 9.6; a second round of 16 rows of 800 takes the GPU 9.3 us, slabs 8.4).
+// One workgroup alone, without slabs and their sum: up to two rounds of rows (16 rows of 800 fp32: 6.2 us on the GPU and
+// 6.3 a call, with slabs 6.4 and 9.8; four rounds, 32 rows: 9.8, with slabs 6.5).
 static bool bwd_alone(int64_t rows, int64_t cols, int vec) {
   if (cols > kMaxHeld) return false;
   const int tpr = row_threads_bwd(cols, vec);
-  return rows <= bwd_block(cols, tpr) / tpr * (tpr == 16 ? 2 : 1);
+  return rows <= bwd_block(cols, tpr, vec) / tpr * 2;
 }
 
 static int64_t bwd_slabs(int64_t rows, int64_t cols, int vec) {
@@ -532,9 +579,9 @@ static int64_t bwd_slabs(int64_t rows, int64_t cols, int vec) {
     return runs < rows ? runs : rows;
   }
   const int tpr = row_threads_bwd(cols, vec);
-  const int64_t per = bwd_block(cols, tpr) / tpr;
+  const int64_t block = bwd_block(cols, tpr, vec), per = block / tpr, most = 1024 / block * kCUs;
   const int64_t need = (rows + per - 1) / per;
-  return need < bwd_most(tpr) ? need : bwd_most(tpr);
+  return need < most ? need : most;
 }
 
 template <typename T, int TPR, int NV, bool SHORT = false> static void launch_fwd(const LnFwd& a, hipStream_t st) {
@@ -548,17 +595,24 @@ template <typename T> static void fwd(const LnFwd& a, hipStream_t st) {
   constexpr int V = Pack<T>::n;
   const int tpr = row_threads_fwd(a.cols, V);
   const int64_t nv = (a.cols + static_cast<int64_t>(tpr) * V - 1) / (static_cast<int64_t>(tpr) * V);
-  if (tpr == 16) {
-    if (a.cols < V) launch_fwd<T, 16, 1, true>(a, st); else if (nv <= 1) launch_fwd<T, 16, 1>(a, st); else launch_fwd<T, 16, 2>(a, st);
+  if (a.cols < V) {
+    launch_fwd<T, 16, 1, true>(a, st);
+  } else if (tpr == 16) {
+    if constexpr (V == 8)
+      if (nv > 2) return nv <= 4 ? launch_fwd<T, 16, 4>(a, st) : launch_fwd<T, 16, 5>(a, st);
+    if (nv <= 1) launch_fwd<T, 16, 1>(a, st); else launch_fwd<T, 16, 2>(a, st);
   } else if (tpr == 64) {
-    if (nv <= 1) launch_fwd<T, 64, 1>(a, st);
-    else if (nv <= 2) launch_fwd<T, 64, 2>(a, st);
-    else if (nv <= 4) launch_fwd<T, 64, 4>(a, st);
-    else launch_fwd<T, 64, 8>(a, st);
+    if constexpr (V == 4)
+      if (nv <= 1) return launch_fwd<T, 64, 1>(a, st);
+    if (nv <= 2) launch_fwd<T, 64, 2>(a, st); else launch_fwd<T, 64, 3>(a, st);
+  } else if (tpr == 128) {
+    if (nv <= 2) launch_fwd<T, 128, 2>(a, st); else if (nv <= 3) launch_fwd<T, 128, 3>(a, st); else launch_fwd<T, 128, 4>(a, st);
   } else if (tpr == 256) {
-    if (nv <= 4) launch_fwd<T, 256, 4>(a, st); else launch_fwd<T, 256, 8>(a, st);
+    if (nv <= 3) launch_fwd<T, 256, 3>(a, st); else launch_fwd<T, 256, 4>(a, st);
+  } else if (tpr == 512) {
+    if (nv <= 3) launch_fwd<T, 512, 3>(a, st); else launch_fwd<T, 512, 4>(a, st);
   } else if (nv <= 4) {
-    launch_fwd<T, 1024, 4>(a, st);
+    if (nv <= 3) launch_fwd<T, 1024, 3>(a, st); else launch_fwd<T, 1024, 4>(a, st);
   } else {
     const int64_t most = 1 << 20;
     hipLaunchKernelGGL((ln_fwd_long_kernel<T>), dim3(static_cast<unsigned>(a.rows < most ? a.rows : most)), dim3(1024), 0,
@@ -575,7 +629,7 @@ template <typename T, int TPR, int NV, int BLOCK = 1024, bool SHORT = false> sta
 }
 
 template <typename T> static int bwd(const LnBwd& a, int64_t slabs, hipStream_t st) {
-  constexpr int V = Pack<T>::n, M = 16 / V;
+  constexpr int V = Pack<T>::n;
   if (a.cols > kMaxHeld) {
     const int64_t most = 1 << 20;
     if (a.dx)
@@ -594,13 +648,14 @@ template <typename T> static int bwd(const LnBwd& a, int64_t slabs, hipStream_t 
   if (tpr == 16) return nv <= 1 ? launch_bwd<T, 16, 1>(a, slabs, st) : launch_bwd<T, 16, 2>(a, slabs, st);
   if (tpr == 64) {
     if (nv <= 1) return launch_bwd<T, 64, 1>(a, slabs, st);
-    if (nv <= 2) return launch_bwd<T, 64, 2>(a, slabs, st);
-    if constexpr (M == 4)
-      if (nv <= 4) return launch_bwd<T, 64, 4>(a, slabs, st);
-    return launch_bwd<T, 64, 2 * M, 512>(a, slabs, st);
+    return nv <= 2 ? launch_bwd<T, 64, 2, 512>(a, slabs, st) : launch_bwd<T, 64, 3, 512>(a, slabs, st);
   }
-  if (tpr == 256) return launch_bwd<T, 256, M, 512>(a, slabs, st);
-  return nv <= M / 2 ? launch_bwd<T, 1024, M / 2>(a, slabs, st) : launch_bwd<T, 1024, M>(a, slabs, st);
+  if (tpr == 128) return launch_bwd<T, 128, 2>(a, slabs, st);
+  if (tpr == 256) return launch_bwd<T, 256, 2, 512>(a, slabs, st);
+  if (tpr == 512) return launch_bwd<T, 512, 2>(a, slabs, st);
+  if constexpr (V == 4)
+    if (nv > 2) return nv <= 3 ? launch_bwd<T, 1024, 3>(a, slabs, st) : launch_bwd<T, 1024, 4>(a, slabs, st);
+  return launch_bwd<T, 1024, 2>(a, slabs, st);
 }
 
 static bool bad_types(int dtype, int wdtype) {
@@ -645,11 +700,11 @@ extern "C" int iadmm_layer_norm_bwd(int64_t rows, int64_t cols, int dtype, int w
   hipStream_t st = static_cast<hipStream_t>(stream);
   const int vec = dtype == IADMM_F32 ? 4 : 8;
   const bool alone = rows > 0 && bwd_alone(rows, cols, vec);
-  const int64_t slabs = bwd_slabs(rows, cols, vec), most = bwd_most(row_threads_bwd(cols, vec));
+  const int64_t slabs = bwd_slabs(rows, cols, vec);
   const LnBwd a{rows, cols, lddy, ldx, dy, x, w, mean, rstd, dx, sums && !alone ? static_cast<float*>(ws) : nullptr,
                 wdtype == IADMM_F32, alone ? dw : nullptr, alone ? db : nullptr};
   if (rows > 0 && (dx || sums)) {
-    const int64_t blocks = alone && sums ? 1 : alone ? (rows < most ? rows : most) : slabs;
+    const int64_t blocks = alone ? (sums ? 1 : rows) : slabs;  // (alone: some hundred rows at most)
     const int rc = dtype == IADMM_F32 ? bwd<float>(a, blocks, st)
                    : dtype == IADMM_BF16 ? bwd<__bf16>(a, blocks, st) : bwd<_Float16>(a, blocks, st);
     if (rc) return rc;

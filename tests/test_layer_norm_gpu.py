@@ -73,7 +73,9 @@ def close(got, want, tol, what):
 
 
 SHAPES = [(16, 800), (17, 800), (32, 1000), (128, 40), (129, 40), (127, 3), (4, 2100), (1, 12000), (2, 12000), (1, 1), (3, 2), (5, 40), (7, 127), (1, 200), (9, 129), (4, 256), (130, 257), (65, 800), (6, 1000),
-          (33, 1025), (300, 7), (1000, 64), (5, 2049), (9, 4097), (3, 9001), (3, 16384), (2, 16385), (5, 20003)]
+          (33, 1025), (300, 7), (1000, 64), (5, 2049), (9, 4097), (3, 9001), (3, 16384), (2, 16385), (5, 20003),
+          (9, 33), (70, 129), (7, 500), (200, 513), (6, 641), (35, 769), (40, 1100), (4, 1536), (19, 1537), (33, 2048), (3, 4095),
+          (600, 2500), (7, 5000), (2, 8192), (3, 8193), (2, 30001)]
 TYPES = [(F32, F32), (BF16, F32), (BF16, BF16), (F16, F32), (F16, F16)]
 
 
@@ -101,6 +103,39 @@ def test_forward_and_gradients(rows, cols, t, wt):
     for name, a, (want, tol) in zip(("dx", "dw", "db"), (dx, dw, db), backward64(dy, x, mean, rstd, None)):
         close(a, want, tol, name + " without weights")
     assert dw.dtype == F32
+
+
+@pytest.mark.parametrize("t", [F32, BF16, F16])
+@pytest.mark.parametrize("cols", [7, 43, 133, 521, 1029, 2051, 5003])
+@pytest.mark.parametrize("where", ["first", "last"])
+def test_infinities_stay_in_their_place(t, cols, where):
+    """A row's last vector overlaps its neighbour: an infinite weight or gradient in the part held twice makes the same
+    infinities and NaN as the formulas, and an infinite x its own row's alone."""
+    from iadmm import ops
+    x, dy, w, b = inputs(5, cols, t, F32)
+    at = 0 if where == "first" else cols - min(cols, 6)
+    _, mean, rstd = ops.layer_norm(x, w, b, stats=True)
+    wi = w.clone()
+    wi[at] = float("inf")
+    got = ops.layer_norm_bwd(dy, x, mean, rstd, wi)
+    want = backward64(dy, x, mean, rstd, wi)
+    assert torch.equal(got[0].isnan(), want[0][0].isnan()) and torch.equal(got[0].isinf(), want[0][0].isinf())
+    plain = ops.layer_norm_bwd(dy, x, mean, rstd, w)
+    assert torch.equal(got[1], plain[1]) and torch.equal(got[2], plain[2])
+    y, clean = ops.layer_norm(x, wi, b), ops.layer_norm(x, w, b)
+    assert bool(y[:, at].isinf().all()) and torch.equal(torch.cat((y[:, :at], y[:, at + 1:]), 1), torch.cat((clean[:, :at], clean[:, at + 1:]), 1))
+    di = dy.clone()
+    di[2, at] = float("inf")
+    dx, dw, db = ops.layer_norm_bwd(di, x, mean, rstd, w)
+    rest = [0, 1, 3, 4]
+    assert torch.equal(dx[rest], plain[0][rest]) and not bool(dx[2].isfinite().any())
+    others = torch.arange(cols, device="cuda") != at
+    assert torch.equal(dw[others], plain[1][others]) and torch.equal(db[others], plain[2][others])
+    assert bool(db[at].isinf()) and not bool(dw[at].isfinite())
+    xi = x.clone()
+    xi[2, at] = float("inf")
+    y, mean, rstd = ops.layer_norm(xi, w, b, stats=True)
+    assert torch.equal(y[rest], clean[rest]) and bool(y[2].isnan().all())
 
 
 @pytest.mark.parametrize("t", [F32, BF16, F16])
