@@ -25,11 +25,11 @@ def test_layer_norm_arguments():
     _abi.call(f, 0, 8, 0, 0, None, 8, None, None, 1e-5, None, None, None, None)                # no rows: nothing to do
     b = "iadmm_layer_norm_bwd"
     need = _abi.lib().iadmm_layer_norm_bwd_ws_bytes(100, 800, 0)
-    assert need == 7 * 2 * 800 * 4                                    # 16 rows a workgroup, dw and db of each
+    assert need == 13 * 2 * 800 * 4                                   # 8 rows a workgroup, dw and db of each
     assert _abi.lib().iadmm_layer_norm_bwd_ws_bytes(10 ** 6, 800, 0) == 256 * 2 * 800 * 4
     assert _abi.lib().iadmm_layer_norm_bwd_ws_bytes(0, 800, 0) == 0
     assert _abi.lib().iadmm_layer_norm_bwd_ws_bytes(16, 800, 0) == 0  # one workgroup has all rows
-    assert _abi.lib().iadmm_layer_norm_bwd_ws_bytes(17, 800, 0) == 2 * 2 * 800 * 4
+    assert _abi.lib().iadmm_layer_norm_bwd_ws_bytes(17, 800, 0) == 3 * 2 * 800 * 4
     refused("bad argument", b, 100, 800, 0, 0, 16, 800, 16, 800, 16, 16, None, 16, 16, 16, 16, need - 4, None)
     refused("bad argument", b, 100, 800, 0, 0, 16, 800, 16, 800, 16, 16, None, 16, 16, 16, None, need, None)
     refused("misaligned", b, 100, 800, 0, 0, 16, 800, 16, 800, 16, 16, None, 16, 16, 16, 20, need, None)
