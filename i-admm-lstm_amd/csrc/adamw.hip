@@ -494,7 +494,7 @@ template <typename T> __global__ void __launch_bounds__(256) adam_decode_kernel(
 
 // ---------------------------------------------------------------------------------------------- the norm
 // sqrt(sum g^2), HBM bound: each workgroup sums a run of neighbouring chunks, one more the workgroups' sums.
-// 100 M bf16 elements in 216 tensors 41 us = 4.9 TB/s, 2.6 M fp32 ones 8 us (two launches).
+// 100 M bf16 elements in 200 tensors 36 us = 5.5 TB/s, 2.6 M fp32 ones 5 us on the GPU and 8.4 a call (two launches).
 struct NormTensor {
   const void* g;
   int64_t n;
@@ -532,14 +532,22 @@ template <typename T, int QUADS> IADMM_DEV double square_sum(const void* g, int6
   return at + QUADS * 1024 <= n ? square_sum_of<T, QUADS, true>(p, at, n) : square_sum_of<T, QUADS, false>(p, at, n);
 }
 
-IADMM_DEV double block_sum_f64(double s, double* red) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o, kWave);
-  if (threadIdx.x % kWave == 0) red[threadIdx.x / kWave] = s;
+// The workgroup's sum, in all its threads: adds whose second operand comes from another lane (a step through LDS waits
+// for some hundred cycles), within 16 lanes, the wave, and over its waves' values (4 or 16).
+template <int CTRL> IADMM_DEV double add_from(double v) {
+  const uint64_t b = static_cast<uint64_t>(__double_as_longlong(v));
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(b), CTRL, 0xF, 0xF, true);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(b >> 32), CTRL, 0xF, 0xF, true);
+  return v + __longlong_as_double(static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo));
+}
+template <int BLOCK> IADMM_DEV double block_sum_f64(double s, double* red) {
+  static_assert(BLOCK == 256 || BLOCK == 1024, "");
+  s = add_from<0x140>(add_from<0x141>(add_from<0x4E>(add_from<0xB1>(s))));  // lanes 1, 2 apart, half rows, rows mirrored
+  s = add_from<0x143>(add_from<0x142>(s));                                  // row_bcast 15, 31: lane 63 has the wave's
+  if (threadIdx.x % kWave == kWave - 1) red[threadIdx.x / kWave] = s;
   __syncthreads();
-  s = red[0];
-  for (unsigned w = 1; w < blockDim.x / kWave; ++w) s += red[w];
-  return s;
+  s = add_from<0x4E>(add_from<0xB1>(red[threadIdx.x % (BLOCK / kWave)]));
+  return BLOCK == 256 ? s : add_from<0x140>(add_from<0x141>(s));
 }
 
 template <int QUADS> __global__ void __launch_bounds__(256) norm_kernel(const NormLaunch a) {
@@ -555,7 +563,7 @@ template <int QUADS> __global__ void __launch_bounds__(256) norm_kernel(const No
     const int64_t at = static_cast<int64_t>(c - t.first) * (QUADS * 1024);
     s += t.half ? square_sum<__bf16, QUADS>(t.g, at, t.n) : square_sum<float, QUADS>(t.g, at, t.n);
   }
-  s = block_sum_f64(s, red);
+  s = block_sum_f64<256>(s, red);
   if (threadIdx.x == 0) a.part[blockIdx.x] = s;
 }
 
@@ -563,15 +571,15 @@ __global__ void __launch_bounds__(1024) norm_end_kernel(const double* part, int 
   __shared__ double red[16];
   double s = 0.0;
   for (int i = threadIdx.x; i < count; i += 1024) s += part[i];
-  s = block_sum_f64(s, red);
+  s = block_sum_f64<1024>(s, red);
   if (threadIdx.x == 0) *norm = static_cast<float>(sqrt(s));
 }
 
 // Workgroups take 2048 elements at a time up to this many in all, 8192 above: 168 000 of them 7.1 us against 7.7 (with the
-// last sum's launch), 2.6 M 8.2 against 8.0.
+// last sum's launch; both since 1 us less), 2.6 M 8.2 against 8.0.
 constexpr int64_t kNormSmall = int64_t{1} << 19;
 // Chunks of 1024 that one workgroup sums alone (16 waves, two rounds): 16 tensors of 2000 elements 5.8 us a call, 8.3 with
-// two launches; with four rounds the GPU takes 7.2 us, the two launches' 5.5.
+// two launches; with four rounds the GPU takes longer than for the two.
 constexpr int64_t kNormFew = 32;
 template <int QUADS> static int launch_norm(NormLaunch& a, hipStream_t st) {  // gives its workgroups
   uint64_t chunks = 0;
@@ -585,9 +593,6 @@ template <int QUADS> static int launch_norm(NormLaunch& a, hipStream_t st) {  //
   return blocks;
 }
 
-// Workgroups of 1024 elements up to this many in all, of 4096 above: 168 000 of them 7.9 us against 8.9 (with the
-// counting launch), 2.6 M 17.9 against 16.6.
-constexpr int64_t kAdamSmall = int64_t{1} << 19;
 // Few elements: one workgroup and one launch, 1024 elements to a wave at a time.
 struct NormFew {
   NormLaunch a;
@@ -613,10 +618,13 @@ __global__ void __launch_bounds__(1024) norm_few_kernel(const NormFew f) {
       }
     }
   }
-  s = block_sum_f64(s, red);
+  s = block_sum_f64<1024>(s, red);
   if (threadIdx.x == 0) *f.norm = static_cast<float>(sqrt(s));
 }
 
+// Workgroups of 1024 elements up to this many in all, of 4096 above: 168 000 of them 7.9 us against 8.9 (with the
+// counting launch), 2.6 M 17.9 against 16.6.
+constexpr int64_t kAdamSmall = int64_t{1} << 19;
 template <bool EIGHT, int QUADS> static void launch_adam(const AdamLaunch& a, const AdamTensor* table, unsigned blocks,
                                                        hipStream_t st) {
   if (table)
