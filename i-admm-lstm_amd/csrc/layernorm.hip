@@ -541,7 +541,7 @@ constexpr int64_t kMaxCols = 1 << 24;  // (ln_slab_kernel's grid has 32 threads 
 constexpr int64_t kMaxHeld = 16384;  // elements of a row that a workgroup of the backward kernel holds
 
 // Forward: threads per row.  Fewer take their sums with less waiting, but each has more to load: up to 3 vectors each
-// in a wave, 4 beyond (1500 columns of fp32: 64 threads 159 us for 400 MB, 128 147, 256 147 with half of them idle; 1200:
+// in a wave, 4 beyond, 8 where there are no more threads (1500 columns of fp32: 64 threads 159 us for 400 MB, 128 147, 256 147 with half of them idle; 1200:
 // 150, 145, 149).  16 threads, whose sums stay among neighbours, with rows of 16 bits up to 5 vectors each (513 columns:
 // 98 us for 200 MB, 64 threads 141; 800 columns: 86 and 82), of 32 bits up to 2 (400 columns: 163 and 139).
 static int row_threads_fwd(int64_t cols, int vec) {
@@ -611,8 +611,8 @@ template <typename T> static void fwd(const LnFwd& a, hipStream_t st) {
     if (nv <= 3) launch_fwd<T, 256, 3>(a, st); else launch_fwd<T, 256, 4>(a, st);
   } else if (tpr == 512) {
     if (nv <= 3) launch_fwd<T, 512, 3>(a, st); else launch_fwd<T, 512, 4>(a, st);
-  } else if (nv <= 4) {
-    if (nv <= 3) launch_fwd<T, 1024, 3>(a, st); else launch_fwd<T, 1024, 4>(a, st);
+  } else if (nv <= 8) {
+    if (nv <= 3) launch_fwd<T, 1024, 3>(a, st); else if (nv <= 4) launch_fwd<T, 1024, 4>(a, st); else launch_fwd<T, 1024, 8>(a, st);
   } else {
     const int64_t most = 1 << 20;
     hipLaunchKernelGGL((ln_fwd_long_kernel<T>), dim3(static_cast<unsigned>(a.rows < most ? a.rows : most)), dim3(1024), 0,

@@ -1,8 +1,8 @@
 """Layer norm (csrc/layernorm.hip) against the formulas in 64 bits.
 
 Tolerances, element by element, with u = 2^-24 (half a step of fp32) and e = half a step of the result's type.
-A sum over a row of n has at most K = 32 + n / 256 roundings on any path (16 elements of a thread, 6 shuffles, at
-most 16 waves; rows above 16384 add n / 1024 elements a thread), so with xh = (x - mu) r, q = dy w:
+A sum over a row of n has at most K = 32 + n / 256 roundings on any path (of a thread 8 + 8 elements and vectors forward,
+16 elements backward, or 24 from n = 1025 on; 6 over a wave, 4 over its waves; rows above 16384 add n / 1024), so with xh = (x - mu) r, q = dy w:
   |mu error| <= K u mean|x|;  r's relative error <= (K / 2 + 8) u;  xh is off by  u (K r mean|x| + (K + 16) |xh|)
   y:   |w| times that, 3 u (|xh w| + |b|) for the last fma and product, and e |y|
   dx (mean and rstd are inputs): r u (K mean|q| + K |xh| mean|q xh| + 8 (|q| + |mean q| + |xh mean(q xh)|)) + e |dx|
@@ -75,7 +75,7 @@ def close(got, want, tol, what):
 SHAPES = [(16, 800), (17, 800), (32, 1000), (128, 40), (129, 40), (127, 3), (4, 2100), (1, 12000), (2, 12000), (1, 1), (3, 2), (5, 40), (7, 127), (1, 200), (9, 129), (4, 256), (130, 257), (65, 800), (6, 1000),
           (33, 1025), (300, 7), (1000, 64), (5, 2049), (9, 4097), (3, 9001), (3, 16384), (2, 16385), (5, 20003),
           (9, 33), (70, 129), (7, 500), (200, 513), (6, 641), (35, 769), (40, 1100), (4, 1536), (19, 1537), (33, 2048), (3, 4095),
-          (600, 2500), (7, 5000), (2, 8192), (3, 8193), (2, 30001)]
+          (600, 2500), (7, 5000), (2, 8192), (3, 8193), (2, 30001), (2, 40000), (2, 70001)]
 TYPES = [(F32, F32), (BF16, F32), (BF16, BF16), (F16, F32), (F16, F16)]
 
 
