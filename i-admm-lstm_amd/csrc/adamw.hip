@@ -570,7 +570,13 @@ template <int QUADS> __global__ void __launch_bounds__(256) norm_kernel(const No
 __global__ void __launch_bounds__(1024) norm_end_kernel(const double* part, int count, float* norm) {
   __shared__ double red[16];
   double s = 0.0;
-  for (int i = threadIdx.x; i < count; i += 1024) s += part[i];
+  for (int i = threadIdx.x; i < count; i += 4096) {  // four loads in flight
+    double v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = part[i + j * 1024 < count ? i + j * 1024 : i];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s += i + j * 1024 < count ? v[j] : 0.0;
+  }
   s = block_sum_f64<1024>(s, red);
   if (threadIdx.x == 0) *norm = static_cast<float>(sqrt(s));
 }
