@@ -37,7 +37,7 @@ namespace iadmm {
 constexpr int kPer = 48;          // tensors that travel in a launch's arguments (3.5 KB of 4)
 constexpr int kPlace = 55;        // tensors that adam_place_kernel's arguments carry (4 KB)
 constexpr int kBlock8 = 256;      // elements under one pair of exponents
-constexpr int kNormPer = 128, kNormBlocks = 1024;
+constexpr int kNormPer = 240, kNormBlocks = 1024;
 
 enum { kHalfP = 1, kHalfG = 2 };  // AdamTensor::flags
 
@@ -494,13 +494,13 @@ template <typename T> __global__ void __launch_bounds__(256) adam_decode_kernel(
 
 // ---------------------------------------------------------------------------------------------- the norm
 // sqrt(sum g^2), HBM bound: each workgroup sums a run of neighbouring chunks, one more the workgroups' sums.
-// 100 M bf16 elements in 200 tensors 36 us = 5.5 TB/s, 2.6 M fp32 ones 5 us on the GPU and 8.4 a call (two launches).
-struct NormTensor {
-  const void* g;
-  int64_t n;
-  uint32_t first;
-  int half;
+// 100 M bf16 elements in 200 tensors 34 us = 5.9 TB/s, 2.6 M fp32 ones 5 us on the GPU and 8.4 a call (two launches).
+struct NormTensor {  // 16 bytes, so that 240 travel in a launch's arguments
+  uint64_t g;      // the address, and the highest bit for bf16
+  uint32_t first;  // its first chunk: all of them are whole up to the next tensor's, but for the last one's
+  uint32_t tail;   // elements
 };
+constexpr uint64_t kHalf = uint64_t{1} << 63;
 struct NormLaunch {
   NormTensor t[kNormPer];
   double* part;
@@ -510,11 +510,11 @@ struct NormLaunch {
 
 // Squares in 64 bits: they neither overflow (fp32's do from 1.8e19 on) nor lose small tensors beside large ones;
 // the conversion and the product cost a third of the time that the bytes take.
-template <typename T, int QUADS, bool FULL> IADMM_DEV double square_sum_of(const T* g, int64_t at, int64_t n) {
+template <typename T, int QUADS, bool FULL> IADMM_DEV double square_sum_of(const T* g, int n) {
   Quad<T> q[QUADS];
 #pragma unroll
   for (int u = 0; u < QUADS; ++u) {
-    const int64_t i = at + u * 1024 + threadIdx.x * 4;
+    const int i = u * 1024 + static_cast<int>(threadIdx.x) * 4;
     q[u] = load_quad<FULL>(g + i, n - i);
   }
   double s = 0.0;
@@ -527,9 +527,15 @@ template <typename T, int QUADS, bool FULL> IADMM_DEV double square_sum_of(const
     }
   return s;
 }
-template <typename T, int QUADS> IADMM_DEV double square_sum(const void* g, int64_t at, int64_t n) {
-  const T* p = static_cast<const T*>(g);
-  return at + QUADS * 1024 <= n ? square_sum_of<T, QUADS, true>(p, at, n) : square_sum_of<T, QUADS, false>(p, at, n);
+template <typename T, int QUADS> IADMM_DEV double square_sum(const T* g, int n) {
+  return n == QUADS * 1024 ? square_sum_of<T, QUADS, true>(g, n) : square_sum_of<T, QUADS, false>(g, n);
+}
+// Chunk c of tensor k: its number of elements; the tensor's address.
+template <int SIZE> IADMM_DEV int chunk_elements(const NormLaunch& a, int k, uint32_t c) {
+  return c + 1 == (k + 1 < a.count ? a.t[k + 1].first : a.chunks) ? static_cast<int>(a.t[k].tail) : SIZE;
+}
+template <typename T> IADMM_DEV const T* chunk_at(const NormTensor& t, int64_t at) {
+  return reinterpret_cast<const T*>(t.g & ~kHalf) + at;
 }
 
 // The workgroup's sum, in all its threads: adds whose second operand comes from another lane (a step through LDS waits
@@ -561,7 +567,9 @@ template <int QUADS> __global__ void __launch_bounds__(256) norm_kernel(const No
     while (k + 1 < a.count && a.t[k + 1].first <= c) ++k;
     const NormTensor& t = a.t[k];
     const int64_t at = static_cast<int64_t>(c - t.first) * (QUADS * 1024);
-    s += t.half ? square_sum<__bf16, QUADS>(t.g, at, t.n) : square_sum<float, QUADS>(t.g, at, t.n);
+    const int n = chunk_elements<QUADS * 1024>(a, k, c);
+    s += t.g & kHalf ? square_sum<__bf16, QUADS>(chunk_at<__bf16>(t, at), n)
+                     : square_sum<float, QUADS>(chunk_at<float>(t, at), n);
   }
   s = block_sum_f64<256>(s, red);
   if (threadIdx.x == 0) a.part[blockIdx.x] = s;
@@ -587,13 +595,19 @@ constexpr int64_t kNormSmall = int64_t{1} << 19;
 // Chunks of 1024 that one workgroup sums alone (16 waves, two rounds): 16 tensors of 2000 elements 5.8 us a call, 8.3 with
 // two launches; with four rounds the GPU takes longer than for the two.
 constexpr int64_t kNormFew = 32;
-template <int QUADS> static int launch_norm(NormLaunch& a, hipStream_t st) {  // gives its workgroups
+static void place_chunks(NormLaunch& a, const int64_t* n, int64_t size) {  // (none is empty)
   uint64_t chunks = 0;
   for (int k = 0; k < a.count; ++k) {
+    const int64_t whole = (n[k] - 1) / size;
     a.t[k].first = static_cast<uint32_t>(chunks);
-    chunks += (static_cast<uint64_t>(a.t[k].n) + QUADS * 1024 - 1) / (QUADS * 1024);
+    a.t[k].tail = static_cast<uint32_t>(n[k] - whole * size);
+    chunks += static_cast<uint64_t>(whole) + 1;
   }
   a.chunks = static_cast<uint32_t>(chunks);
+}
+template <int QUADS> static int launch_norm(NormLaunch& a, const int64_t* n, hipStream_t st) {  // gives its workgroups
+  place_chunks(a, n, QUADS * 1024);
+  const uint32_t chunks = a.chunks;
   const int blocks = chunks < kNormBlocks ? static_cast<int>(chunks) : kNormBlocks;
   hipLaunchKernelGGL(norm_kernel<QUADS>, dim3(blocks), dim3(256), 0, st, a);
   return blocks;
@@ -604,21 +618,23 @@ struct NormFew {
   NormLaunch a;
   float* norm;
 };
+static_assert(sizeof(NormFew) <= 4096, "a launch's arguments");
 __global__ void __launch_bounds__(1024) norm_few_kernel(const NormFew f) {
   __shared__ double red[16];
   const int lane = threadIdx.x % kWave;
   double s = 0.0;
   for (uint32_t c = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave); c < f.a.chunks; c += 16) {
-    const NormTensor& t = f.a.t[find_tensor(f.a.t, f.a.count, c)];
+    const int k = find_tensor(f.a.t, f.a.count, c), n = chunk_elements<1024>(f.a, k, c);
+    const NormTensor& t = f.a.t[k];
     const int64_t at = static_cast<int64_t>(c - t.first) * 1024;
     for (int u = 0; u < 4; ++u) {
-      const int64_t i = at + u * 256 + lane * 4;
-      if (t.half) {
-        const Quad<__bf16> q = load_quad(static_cast<const __bf16*>(t.g) + i, t.n - i);
+      const int i = u * 256 + lane * 4;
+      if (t.g & kHalf) {
+        const Quad<__bf16> q = load_quad(chunk_at<__bf16>(t, at) + i, n - i);
 #pragma unroll
         for (int j = 0; j < 4; ++j) s = fma(static_cast<float>(q.v[j]), static_cast<double>(static_cast<float>(q.v[j])), s);
       } else {
-        const Quad<float> q = load_quad(static_cast<const float*>(t.g) + i, t.n - i);
+        const Quad<float> q = load_quad(chunk_at<float>(t, at) + i, n - i);
 #pragma unroll
         for (int j = 0; j < 4; ++j) s = fma(static_cast<double>(q.v[j]), static_cast<double>(q.v[j]), s);
       }
@@ -661,35 +677,33 @@ extern "C" int iadmm_grad_norm(int64_t count, const iadmm_grad_tensor* grads, fl
   hipStream_t st = static_cast<hipStream_t>(stream);
   double* part = static_cast<double*>(ws);
   int parts = 0;
-  NormLaunch a;
+  NormFew f;
+  NormLaunch& a = f.a;
+  int64_t n[kNormPer], total = 0, few = 0, filled = 0;
+  for (int64_t i = 0; i < count; ++i) few += (grads[i].n + 1023) / 1024, filled += grads[i].n > 0;
+  const bool alone = filled <= kNormPer && few <= kNormFew;
   a.count = 0;
-  int64_t total = 0, few = 0;
-  for (int64_t i = 0; i < count; ++i) few += (grads[i].n + 1023) / 1024;
-  if (count <= kNormPer && few <= kNormFew) {
-    NormFew f;
-    f.norm = norm, f.a.count = 0, f.a.part = nullptr, f.a.chunks = static_cast<uint32_t>(few);
-    uint32_t first = 0;
-    for (int64_t i = 0; i < count; ++i) {
-      f.a.t[f.a.count++] = NormTensor{grads[i].g, grads[i].n, first, grads[i].dtype == IADMM_BF16};
-      first += static_cast<uint32_t>((grads[i].n + 1023) / 1024);
-    }
-    hipLaunchKernelGGL(norm_few_kernel, dim3(1), dim3(1024), 0, st, f);
-    IADMM_CHECK_LAUNCH();
-    return IADMM_OK;
-  }
   for (int64_t i = 0; i < count; ++i) {
     if (grads[i].n > 0) {
-      a.t[a.count++] = NormTensor{grads[i].g, grads[i].n, 0u, grads[i].dtype == IADMM_BF16};
+      n[a.count] = grads[i].n;
+      a.t[a.count++] = NormTensor{reinterpret_cast<uint64_t>(grads[i].g) | (grads[i].dtype == IADMM_BF16 ? kHalf : 0), 0u, 0u};
       total += grads[i].n;
     }
-    if (a.count > 0 && (a.count == kNormPer || i == count - 1)) {
+    if (!alone && a.count > 0 && (a.count == kNormPer || i == count - 1)) {
       a.part = part + parts;
-      const int blocks = total <= kNormSmall ? launch_norm<2>(a, st) : launch_norm<8>(a, st);
+      const int blocks = total <= kNormSmall ? launch_norm<2>(a, n, st) : launch_norm<8>(a, n, st);
       IADMM_CHECK_LAUNCH();
       parts += blocks;
       a.count = 0;
       total = 0;
     }
+  }
+  if (alone) {
+    place_chunks(a, n, 1024);
+    a.part = nullptr, f.norm = norm;
+    hipLaunchKernelGGL(norm_few_kernel, dim3(1), dim3(1024), 0, st, f);
+    IADMM_CHECK_LAUNCH();
+    return IADMM_OK;
   }
   hipLaunchKernelGGL(norm_end_kernel, dim3(1), dim3(1024), 0, st, part, parts, norm);
   IADMM_CHECK_LAUNCH();

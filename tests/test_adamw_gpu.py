@@ -413,7 +413,8 @@ def test_counts_on_the_device(eight):
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_grad_norm(dtype):
     from iadmm import ops
-    for sizes in ([300] * 16, [1024] * 32, [1024] * 31 + [1025], [0, 3, 0, 2049], [1] * 32, [1] * 33, [1], [5], [8192], [8193], [100003, 0, 3], [(i * 97) % 3000 for i in range(300)], [30_000_001]):
+    for sizes in ([300] * 16, [1024] * 32, [1024] * 31 + [1025], [0, 3, 0, 2049], [1] * 32, [1] * 33, [1], [5], [8192], [8193], [100003, 0, 3], [(i * 97) % 3000 for i in range(300)], [30_000_001],
+                  [(i * 1931) % 40000 for i in range(240)], [8192] * 241, [5] * 480, [16384, 16383, 0, 16385, 2048, 600_000], [0, 0]):
         g = torch.Generator(device="cuda").manual_seed(len(sizes))
         G = [(10.0 ** (k % 7 - 3) * torch.randn(n, device="cuda", generator=g)).to(dtype) for k, n in enumerate(sizes)]
         want = math.sqrt(sum(float(x.double().square().sum()) for x in G))
