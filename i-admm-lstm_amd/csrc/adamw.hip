@@ -493,8 +493,9 @@ template <typename T> __global__ void __launch_bounds__(256) adam_decode_kernel(
 }
 
 // ---------------------------------------------------------------------------------------------- the norm
-// sqrt(sum g^2), HBM bound: each workgroup sums a run of neighbouring chunks, one more the workgroups' sums.
-// 100 M bf16 elements in 200 tensors 34 us = 5.9 TB/s, 2.6 M fp32 ones 5 us on the GPU and 8.4 a call (two launches).
+// sqrt(sum g^2), HBM bound: the workgroups sum every 1024th chunk, so that neighbouring ones are read at the same time (a
+// run of neighbours each: 400 M fp32 282 us, now 258), one more the workgroups' sums.
+// 100 M bf16 elements in 200 tensors 33 us = 6.1 TB/s, 2.6 M fp32 ones 5 us on the GPU and 8.4 a call (two launches).
 struct NormTensor {  // 16 bytes, so that 240 travel in a launch's arguments
   uint64_t g;      // the address, and the highest bit for bf16
   uint32_t first;  // its first chunk: all of them are whole up to the next tensor's, but for the last one's
@@ -530,9 +531,9 @@ template <typename T, int QUADS, bool FULL> IADMM_DEV double square_sum_of(const
 template <typename T, int QUADS> IADMM_DEV double square_sum(const T* g, int n) {
   return n == QUADS * 1024 ? square_sum_of<T, QUADS, true>(g, n) : square_sum_of<T, QUADS, false>(g, n);
 }
-// Chunk c of tensor k: its number of elements; the tensor's address.
-template <int SIZE> IADMM_DEV int chunk_elements(const NormLaunch& a, int k, uint32_t c) {
-  return c + 1 == (k + 1 < a.count ? a.t[k + 1].first : a.chunks) ? static_cast<int>(a.t[k].tail) : SIZE;
+// Chunk c of a tensor whose successor's first is `next` (or that of all behind it): its number of elements.
+template <int SIZE> IADMM_DEV int chunk_elements(const NormTensor& t, uint32_t next, uint32_t c) {
+  return c + 1 == next ? static_cast<int>(t.tail) : SIZE;
 }
 template <typename T> IADMM_DEV const T* chunk_at(const NormTensor& t, int64_t at) {
   return reinterpret_cast<const T*>(t.g & ~kHalf) + at;
@@ -556,18 +557,22 @@ template <int BLOCK> IADMM_DEV double block_sum_f64(double s, double* red) {
   return BLOCK == 256 ? s : add_from<0x140>(add_from<0x141>(s));
 }
 
+// The launch's tensors lie in LDS, as a chunk's is looked for each time: four ballots (from the arguments 40 us for 33).
 template <int QUADS> __global__ void __launch_bounds__(256) norm_kernel(const NormLaunch a) {
   __shared__ double red[4];
-  // a run of neighbouring chunks, so that the tensor is looked for once
-  uint32_t c = static_cast<uint32_t>(static_cast<uint64_t>(a.chunks) * blockIdx.x / gridDim.x);
-  const uint32_t end = static_cast<uint32_t>(static_cast<uint64_t>(a.chunks) * (blockIdx.x + 1) / gridDim.x);
-  int k = find_tensor(a.t, a.count, c);
+  __shared__ NormTensor table[256 + 1];
+  static_assert(kNormPer <= 256, "one entry per thread");
+  const int lane = threadIdx.x % kWave;
+  for (int i = threadIdx.x; i < 256 + 1; i += 256) table[i] = i < a.count ? a.t[i] : NormTensor{0, a.chunks, 0};
+  __syncthreads();
   double s = 0.0;
-  for (; c < end; ++c) {
-    while (k + 1 < a.count && a.t[k + 1].first <= c) ++k;
-    const NormTensor& t = a.t[k];
+  for (uint32_t c = blockIdx.x; c < a.chunks; c += gridDim.x) {
+    int k = -1;
+#pragma unroll
+    for (int j = 0; j < 256; j += kWave) k += __popcll(__ballot(table[j + lane].first <= c));
+    const NormTensor t = table[k];
     const int64_t at = static_cast<int64_t>(c - t.first) * (QUADS * 1024);
-    const int n = chunk_elements<QUADS * 1024>(a, k, c);
+    const int n = __builtin_amdgcn_readfirstlane(chunk_elements<QUADS * 1024>(t, table[k + 1].first, c));
     s += t.g & kHalf ? square_sum<__bf16, QUADS>(chunk_at<__bf16>(t, at), n)
                      : square_sum<float, QUADS>(chunk_at<float>(t, at), n);
   }
@@ -624,8 +629,9 @@ __global__ void __launch_bounds__(1024) norm_few_kernel(const NormFew f) {
   const int lane = threadIdx.x % kWave;
   double s = 0.0;
   for (uint32_t c = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave); c < f.a.chunks; c += 16) {
-    const int k = find_tensor(f.a.t, f.a.count, c), n = chunk_elements<1024>(f.a, k, c);
+    const int k = find_tensor(f.a.t, f.a.count, c);
     const NormTensor& t = f.a.t[k];
+    const int n = chunk_elements<1024>(t, k + 1 < f.a.count ? f.a.t[k + 1].first : f.a.chunks, c);
     const int64_t at = static_cast<int64_t>(c - t.first) * 1024;
     for (int u = 0; u < 4; ++u) {
       const int i = u * 256 + lane * 4;
