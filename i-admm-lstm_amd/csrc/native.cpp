@@ -356,6 +356,25 @@ PyObject* py_grad_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// The bytes of a tensor, and whether the call writes them.
+struct Held {
+  uintptr_t from, to;
+  bool written;
+  Held(const void* p, int64_t bytes, bool w)
+      : from(reinterpret_cast<uintptr_t>(p)), to(from + static_cast<uintptr_t>(bytes)), written(w) {}
+};
+// Whether what is written overlaps nothing else.
+bool apart(std::vector<Held>& held) {
+  std::sort(held.begin(), held.end(), [](const Held& a, const Held& b) { return a.from < b.from; });
+  uintptr_t all = 0, written = 0;  // where the tensors so far end
+  for (const Held& h : held) {
+    if (h.from < (h.written ? all : written)) return false;
+    all = std::max(all, h.to);
+    if (h.written) written = std::max(written, h.to);
+  }
+  return true;
+}
+
 // adamw_step(params, grads, exp_avgs, exp_avg_sqs, exponents, step, lr, beta1, beta2, eps, weight_decay, norm,
 //            max_norm, seed); step: a number, a list of them or an int64 tensor
 PyObject* py_adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -404,8 +423,8 @@ PyObject* py_adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
   int64_t step = 0;
   if (!counted && !numbers) step = PyLong_AsLongLong(a[5]);
   std::vector<iadmm_adamw_tensor> rec(use.size());
-  std::vector<const void*> held;
-  held.reserve(use.size() * 4);
+  std::vector<Held> held;
+  held.reserve(use.size() * 5);
   for (size_t k = 0; k < use.size(); ++k) {
     const int64_t size = p.t[k].numel();
     TORCH_CHECK_VALUE(g.t[k].sizes() == p.t[k].sizes(), "gradient ", use[k], " is ", g.t[k].sizes(), ", its parameter ",
@@ -428,13 +447,16 @@ PyObject* py_adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
     r.slot = use[k];
     r.dtype = static_cast<int16_t>(type_code(p.t[k].scalar_type()));
     r.gdtype = static_cast<int16_t>(type_code(g.t[k].scalar_type()));
-    for (const void* q : {static_cast<const void*>(r.p), static_cast<const void*>(r.m), static_cast<const void*>(r.v),
-                          static_cast<const void*>(r.e)})
-      if (q) held.push_back(q);
+    if (size > 0) {
+      const int64_t moments = size * (eight ? 1 : 4);
+      held.emplace_back(r.p, size * (r.dtype ? 2 : 4), true);
+      held.emplace_back(r.g, size * (r.gdtype ? 2 : 4), false);
+      held.emplace_back(r.m, moments, true);
+      held.emplace_back(r.v, moments, true);
+      if (eight) held.emplace_back(r.e, (size + 255) / 256 * 2, true);
+    }
   }
-  std::sort(held.begin(), held.end());
-  TORCH_CHECK_VALUE(std::adjacent_find(held.begin(), held.end()) == held.end(),
-                    "a parameter or its state is in the lists twice");
+  TORCH_CHECK_VALUE(apart(held), "a parameter or its state is in the lists twice, or overlaps another tensor of the call");
   const int64_t many = static_cast<int64_t>(rec.size()), bytes = abi.adamw_ws_bytes(many);
   const at::AutoGradMode off(false);
   Tensor ws = counted || many > 48 ? f32_on(p.t[0], {bytes / 4}) : Tensor();  // (include/iadmm.h: when it is used)
@@ -443,7 +465,7 @@ PyObject* py_adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
        abi.adamw_step(many, rec.data(), eight ? 8 : 32, lr, lr_dev.defined() ? lr_dev.const_data_ptr<float>() : nullptr, b1, b2,
                       eps, decay, norm.defined() ? norm.const_data_ptr<float>() : nullptr, most, seed,
                       counted ? counts.mutable_data_ptr<int64_t>() : nullptr, address_of(ws), bytes, stream_of(p.device)));
-  for (const List* l : {&p, &m, &v})
+  for (const List* l : {&p, &m, &v, &e})
     for (const Tensor& t : l->t) written(t);
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS

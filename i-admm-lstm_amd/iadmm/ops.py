@@ -593,7 +593,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9, 
     ``norm`` (0-dim fp32 device tensor, :func:`grad_norm`) with ``max_norm``: the gradients count as scaled by
     min(1, max_norm / (norm + 1e-6)); they themselves stay as they are.
 
-    No two tensors of the call may overlap.  A call with an error changes nothing."""
+    What the call writes may overlap no other tensor of it (refused); gradients may be shared.  A call with an error changes nothing."""
     if (not isinstance(step, torch.Tensor) and len(params) and getattr(params[0], "is_cuda", False)
             and torch.cuda.is_current_stream_capturing()):
         raise RuntimeError("a captured step needs its count on the device (an int64 tensor as step): a number "

@@ -391,7 +391,7 @@ int iadmm_layer_norm_bwd(int64_t rows, int64_t cols, int dtype, int wdtype, cons
  *     state_bits 32: m, v are fp32.  state_bits 8: m, v hold n codes of 8 bits, e holds two int8 exponents
  *     for each 256 elements (ceil(n / 256) pairs; all zero is a state of zeros); codes are rounded up or
  *     down at random, as bf16 parameters are, by (seed, step, slot, element).  dtype / gdtype: IADMM_F32
- *     or IADMM_BF16.  No two tensors of a call may overlap.
+ *     or IADMM_BF16.  Nothing that the call writes may overlap another tensor of it.
  *     step: the step that this call makes, counted from 1; or, with steps_dev, steps_dev[slot] is raised by
  *     1 and used (a captured call then counts its replays); lr_dev (needs steps_dev), where not NULL,
  *     replaces lr.  ws: iadmm_adamw_ws_bytes(count) bytes, 16-B aligned, with steps_dev or more than 48 tensors.

@@ -518,6 +518,29 @@ def test_refusals_change_nothing():
     assert all(torch.equal(a, b) for a, b in zip(keep, P + M + V))
 
 
+def test_overlapping_tensors_are_refused():
+    """Parts of one buffer that reach into each other, a gradient that reaches into what is written; parts side by side
+    and gradients that share theirs (which is only read) are taken."""
+    from iadmm import ops
+    buf, g = torch.randn(1000, device="cuda"), torch.randn(400, device="cuda")
+    m, v = ([torch.zeros(300, device="cuda") for _ in range(2)] for _ in range(2))
+    keep = buf.clone()
+    P = [buf[:300], buf[299:599]]
+    with pytest.raises(ValueError, match="overlaps"):
+        ops.adamw_step(P, [g[:300], g[:300]], m, v, 1)
+    with pytest.raises(ValueError, match="overlaps"):
+        ops.adamw_step([buf[:300], buf[300:600]], [buf[599:899], g[:300]], m, v, 1)
+    with pytest.raises(ValueError, match="overlaps"):
+        ops.adamw_step([buf[:300], buf[300:600]], [g[:300], g[:300]], [m[0], buf[500:800]], v, 1)
+    torch.cuda.synchronize()
+    assert torch.equal(buf, keep)
+    ops.adamw_step([buf[:300], buf[300:600]], [buf[600:900], g[50:350]], m, v, 1)
+    a, b = keep[:300].clone(), keep[300:600].clone()
+    n, w = ([torch.zeros(300, device="cuda") for _ in range(2)] for _ in range(2))
+    ops.adamw_step([a, b], [keep[600:900].clone(), g[50:350].clone()], n, w, 1)
+    assert torch.equal(buf, torch.cat((a, b, keep[600:])))
+
+
 def test_numbers_of_numpy():
     from iadmm import ops
     A, C = tensors([100]), tensors([100])
