@@ -1,6 +1,6 @@
 #!/bin/bash
 # r06: tests touched by the ADVICE fixes (two L11^-1 buffers, B=512 split vs rank-128); the batch-2 recipe
-# window measured (wall, cProfile, rocprof kernel trace); the LU capture probe on the guard-free variant
+# window measured (wall, cProfile, rocprof kernel trace)
 set -o pipefail
 mkdir -p gpurun_out
 export TMPDIR=/tmp
@@ -14,7 +14,3 @@ timeout -k 10 300 python3 -u -m cProfile -o gpurun_out/r06b_b2.prof bench_train.
 python3 -c "import pstats; pstats.Stats('gpurun_out/r06b_b2.prof').sort_stats('tottime').print_stats(25)" > gpurun_out/r06b_b2_cprofile.txt 2>&1
 timeout -k 10 300 rocprofv3 --kernel-trace --stats -d gpurun_out/r06b_prof -o b2 -- python3 bench_train.py --batch 2 --micro_batch 2 --steps 1 --warmup 1 > gpurun_out/r06b_b2_prof.log 2>&1 || exit 4
 find gpurun_out/r06b_prof -name "*stats*" | head
-IADMM_LIB_PATH=$PWD/tools/var_lu_capture.so timeout -k 10 300 python3 -u tools/lu_capture_probe.py > gpurun_out/r06b_capture_probe.log 2>&1
-rc=$?
-cat gpurun_out/r06b_capture_probe.log | tail -20
-exit $rc

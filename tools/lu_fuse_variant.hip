@@ -2139,8 +2139,8 @@ static int lu_factor_blocks(int64_t B, int64_t N, float* A, int* piv, int* info,
   // strips fork from it directly (r06).  The eager hop s0 -> s1 -> s2 is a fork from a stream that
   // joined the capture through another forked stream, and the HIP runtime python processes load --
   // PyTorch's bundled libamdhip64 (ROCm 7.0.2), which this library binds to by soname -- crashes in
-  // hipStreamEndCapture on exactly that shape (tools/capture_probe.hip variant 2; variants 1, 9, 10,
-  // forks from the capture's origin only, capture and replay; the system HIP 7.2 runtime takes all of
+  // hipStreamEndCapture on exactly that shape (variant 2 of
+  // the measured stream patterns; forks from the capture's origin only, variants 1, 9 and 10, capture and replay; the system HIP 7.2 runtime takes all of
   // them: profiles/r06_capture_probe.txt).  r05 ran the whole factorization on one stream under
   // capture instead; the captured graph now has the eager schedule's concurrency.  (Stream
   // priorities do not carry into a graph, so s1's role is moot there.)
@@ -2487,8 +2487,8 @@ extern "C" int iadmm_lu_factor_ex(int64_t B, int64_t N, float* A, int* piv, int*
   // two streams -- the instances share nothing, so the factors are bit for bit those of one call, and
   // one half's latency-bound panel steps overlap the other half's updates (B = 1024, N = 2000: 75.8 ->
   // 74.1 ms, profiles/r05_lu_split_ab.txt; four parts: 78.7).  Both halves fork from the caller's stream
-  // by one event, which a stream capture takes as well (tools/capture_probe.hip variant 9; r06 -- r05
-  // kept captured factorizations on one stream).
+  // by one event, which a stream capture takes as well (r05 kept captured factorizations on one
+  // stream).
   const bool split = ctx && pairs && gather && N <= kLeftDeferMaxN && N % 4 == 0 && aligned16(A) && B >= 512 &&
                      ws_bytes >= lu_ws_bytes(B / 2, N) + lu_ws_bytes(B - B / 2, N);
   if (!split) return run(0, B, static_cast<char*>(ws), s, ctx);
