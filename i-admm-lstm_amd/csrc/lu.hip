@@ -2034,9 +2034,9 @@ static int lu_rank64(int64_t B, int64_t N, int K0, int cend, int cmax, float* A,
 // them in library statics behind a mutex, against the header's contract).  s1 carries the critical
 // path -- the block factorizations and the strips the next block needs -- and s2 the rest of each
 // trailing update, both at the default priority (work on streams of different priorities has hung on
-// this runtime; it had been worth 1 % here, 81.1 -> 80.2 ms).  The caller's stream forks into s1 and joins it at the end; every path out of
-// lu_factor_blocks after the fork runs that join (the caller may free A, piv and ws on its stream
-// as soon as the call returns).
+// this runtime; it had been worth 1 % here, 81.1 -> 80.2 ms).  The caller's stream forks into s1 and
+// joins it at the end; every path out of lu_factor_blocks after the fork runs that join (the caller may
+// free A, piv and ws on its stream as soon as the call returns).
 struct iadmm_lu_ctx {
   int device = -1;
   hipStream_t s1 = nullptr, s2 = nullptr;
@@ -2081,9 +2081,9 @@ static int lu_factor_blocks(int64_t B, int64_t N, float* A, int* piv, int* info,
   // strips fork from it directly (r06).  The eager hop s0 -> s1 -> s2 is a fork from a stream that
   // joined the capture through another forked stream, and the HIP runtime python processes load --
   // PyTorch's bundled libamdhip64 (ROCm 7.0.2), which this library binds to by soname -- crashes in
-  // hipStreamEndCapture on exactly that shape (variant 2 of
-  // the measured stream patterns; forks from the capture's origin only, variants 1, 9 and 10, capture and replay; the system HIP 7.2 runtime takes all of
-  // them: profiles/r06_capture_probe.txt).  r05 ran the whole factorization on one stream under
+  // hipStreamEndCapture on exactly that shape (variant 2 of the measured stream patterns; forks from the
+  // capture's origin only, variants 1, 9 and 10, capture and replay; the system HIP 7.2 runtime takes all
+  // of them: profiles/r06_capture_probe.txt).  r05 ran the whole factorization on one stream under
   // capture instead; the captured graph now has the eager schedule's concurrency.
   bool capturing = false;
   if (side) {
