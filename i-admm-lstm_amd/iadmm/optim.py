@@ -41,8 +41,17 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"betas {betas}, eps {eps} or weight_decay {weight_decay} is out of range")
         self.state_bits, self.max_norm, self.seed, self.capturable = state_bits, max_norm, int(seed), bool(capturable)
         self.norm = None
-        self._counts = {}  # group index -> int64 device tensor: the steps made, one per parameter (capturable)
+        self._counts = {}  # group index -> int64 device tensor of the steps made, and its elements by parameter (capturable)
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+
+    def __getstate__(self):
+        """What a copy or a pickle holds: torch's entries and this optimizer's own settings (torch keeps its own alone)."""
+        own = ("state_bits", "max_norm", "seed", "capturable", "norm")
+        return {**super().__getstate__(), **{k: getattr(self, k) for k in own}}
+
+    def __setstate__(self, state):
+        super().__setstate__(state)  # (load_state_dict comes here too, with the state and the groups)
+        self._counts = {}            # the next step gathers them from the parameters' "step"
 
     def add_param_group(self, group):
         super().add_param_group(group)
