@@ -75,15 +75,17 @@ class AdamW(torch.optim.Optimizer):
 
     def _count(self, gi, params):
         """The group's steps as one device tensor, whose elements the parameters' "step" entries are."""
-        counts = self._counts.get(gi)
-        if counts is None or counts.numel() != len(params) or counts.device != params[0].device or any(
-                not isinstance(self.state[p].get("step", 0), torch.Tensor) for p in params):
+        counts, own = self._counts.get(gi, (None, ()))
+        # (a copy of this optimizer, a changed group or a state put in from outside: entries that are not these elements)
+        if len(own) != len(params) or any(self.state[p].get("step") is not c for p, c in zip(params, own)):
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("make one step before the capture: the steps' counts are not on the device yet")
             made = [int(self.state[p].get("step", 0)) for p in params]
-            counts = self._counts[gi] = torch.tensor(made, dtype=torch.int64, device=params[0].device)
-            for i, p in enumerate(params):
-                self.state[p]["step"] = counts[i]
+            counts = torch.tensor(made, dtype=torch.int64, device=params[0].device)
+            own = counts.unbind()
+            self._counts[gi] = counts, own
+            for p, c in zip(params, own):
+                self.state[p]["step"] = c
         return counts
 
     @torch.no_grad()

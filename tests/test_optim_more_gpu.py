@@ -50,3 +50,27 @@ def test_a_copy_goes_on_as_its_original(copied, bits, capturable):
     for p, q in zip(a, b):
         assert int(opt.state[p]["step"]) == int(other.state[q]["step"]) == 5
         assert all(torch.equal(x, y) for x, y in zip(opt.moments(p), other.moments(q)))
+
+
+def test_counts_follow_the_parameters_not_their_place():
+    """Counts on the device after the groups changed places, and beside a shallow copy that steps the same parameters:
+    the same bits as an optimizer that counts on the host, whose counts are the parameters' own."""
+    from iadmm.optim import AdamW
+    ends = []
+    for capturable in (False, True):
+        a = params()
+        opt = AdamW([dict(params=a[:1]), dict(params=a[1:2])], lr=1e-2, betas=(0.5, 0.75), capturable=capturable)
+        set_grads(a[:1], 0)
+        opt.step()
+        for t in range(1, 6):
+            set_grads(a[:2], t)
+            opt.step()
+            if t == 2:
+                opt.param_groups.reverse()
+            if t == 3:
+                shallow = copy.copy(opt)
+                shallow.step()
+        assert [int(opt.state[p]["step"]) for p in a[:2]] == [7, 6]
+        ends.append([p.detach().clone() for p in a[:2]])
+    for p, q in zip(*ends):  # (the corrections of the two kinds of counts are rounded apart: 2 u of an update, 7 updates)
+        assert bool(((p - q).abs() <= 7 * 2.0 ** -24 * (4 * p.abs() + 24 * 2e-2)).all())
