@@ -54,12 +54,16 @@ class AdamW(torch.optim.Optimizer):
         self._counts = {}            # the next step gathers them from the parameters' "step"
 
     def add_param_group(self, group):
-        super().add_param_group(group)
-        for p in self.param_groups[-1]["params"]:
-            if p.dtype not in (torch.float32, torch.bfloat16):
-                raise TypeError(f"parameters must be float32 or bfloat16, got {p.dtype}")
-            if not p.is_contiguous():
-                raise ValueError(f"parameters must be contiguous, got strides {p.stride()} for {tuple(p.shape)}")
+        super().add_param_group(group)  # (params may be a generator: looked at where they are a list)
+        try:
+            for p in self.param_groups[-1]["params"]:
+                if p.dtype not in (torch.float32, torch.bfloat16):
+                    raise TypeError(f"parameters must be float32 or bfloat16, got {p.dtype}")
+                if not p.is_contiguous():
+                    raise ValueError(f"parameters must be contiguous, got strides {p.stride()} for {tuple(p.shape)}")
+        except (TypeError, ValueError):
+            self.param_groups.pop()
+            raise
 
     def _state(self, p):
         """The state of one parameter, zeros at first."""

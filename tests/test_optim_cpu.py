@@ -26,3 +26,17 @@ def test_a_copied_optimizer_has_its_settings_and_steps(copied):
     other.param_groups[0]["params"][0].grad = torch.ones(3)
     with pytest.raises(ValueError, match="no CPU fallback"):
         other.step()
+
+
+@pytest.mark.parametrize("bad,error", [(lambda: torch.nn.Parameter(torch.zeros(3, dtype=torch.float16)), TypeError),
+                                       (lambda: torch.nn.Parameter(torch.zeros(3, 4).t()), ValueError)])
+def test_a_refused_group_is_not_added(bad, error):
+    opt = AdamW([parameter()])
+    p = bad()
+    with pytest.raises(error):
+        opt.add_param_group(dict(params=(q for q in (parameter(2), p))))
+    assert len(opt.param_groups) == 1
+    p.grad = torch.ones_like(p)
+    assert opt.step() is None                       # the refused parameter is not the optimizer's
+    opt.add_param_group(dict(params=[parameter(2)], lr=0.1))
+    assert [g["lr"] for g in opt.param_groups] == [1e-3, 0.1]
