@@ -24,8 +24,8 @@ class AdamW(torch.optim.Optimizer):
     ``lr`` of its capture unless ``lr`` is a 1-element fp32 device tensor.
 
     Parameters without a gradient are left alone, as torch.optim does.  ``state_dict`` has torch.optim.AdamW's
-    entries ("step", "exp_avg", "exp_avg_sq"; with 8 bits "exponents" too), and a state of torch.optim.Adam or
-    AdamW loads into 32 bits."""
+    entries ("step", "exp_avg", "exp_avg_sq"; with 8 bits "exponents" too), and a state of torch.optim.AdamW, or of
+    Adam without weight decay, loads into 32 bits."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, state_bits=32, max_norm=None,
                  seed=0, capturable=False):
@@ -143,6 +143,8 @@ class AdamW(torch.optim.Optimizer):
               for p, i in zip(group["params"], saved["params"])]
         if any(g.get("maximize") or g.get("amsgrad") for g in state_dict["param_groups"]):
             raise ValueError("a state of an optimizer with maximize or amsgrad does not load")
+        if any(g.get("weight_decay") and g.get("decoupled_weight_decay", True) is False for g in state_dict["param_groups"]):
+            raise ValueError("a state of Adam with a weight decay inside its gradients does not load: the decay is decoupled here")
         for p, s in of:
             if s is None or not s:
                 continue
@@ -154,6 +156,8 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError(f"a state of {tuple(s['exp_avg'].shape)} does not fit a parameter of {tuple(p.shape)}")
         super().load_state_dict(state_dict)
         self._counts = {}
+        for g in self.param_groups:  # (Adam's mark: without a decay it loads, and the group is AdamW's from here on)
+            g.pop("decoupled_weight_decay", None)
         for p, s in of:
             if s is None or not s:
                 continue

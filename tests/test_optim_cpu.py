@@ -40,3 +40,32 @@ def test_a_refused_group_is_not_added(bad, error):
     assert opt.step() is None                       # the refused parameter is not the optimizer's
     opt.add_param_group(dict(params=[parameter(2)], lr=0.1))
     assert [g["lr"] for g in opt.param_groups] == [1e-3, 0.1]
+
+
+def stepped(kind, **kw):
+    """A torch optimizer after one step, and a copy of its parameter."""
+    p = parameter()
+    opt = kind([p], **kw)
+    p.grad = torch.ones(3)
+    opt.step()
+    return opt, torch.nn.Parameter(p.detach().clone())
+
+
+def test_a_decay_inside_the_gradient_does_not_become_a_decoupled_one():
+    """torch.optim.Adam's weight decay enters the moments; AdamW's does not."""
+    ref, p = stepped(torch.optim.Adam, weight_decay=0.1)
+    opt = AdamW([p], lr=0.25)
+    with pytest.raises(ValueError, match="decoupled"):
+        opt.load_state_dict(ref.state_dict())
+    assert opt.param_groups[0]["lr"] == 0.25 and not opt.state
+    for kind, kw in ((torch.optim.Adam, {}), (torch.optim.Adam, dict(weight_decay=0.1, decoupled_weight_decay=True)),
+                     (torch.optim.AdamW, dict(weight_decay=0.1))):
+        ref, p = stepped(kind, **kw)
+        opt = AdamW([p], lr=0.25)
+        opt.load_state_dict(ref.state_dict())
+        assert opt.param_groups[0]["weight_decay"] == kw.get("weight_decay", 0.0)
+        assert torch.equal(opt.state[p]["exp_avg"], next(iter(ref.state.values()))["exp_avg"]) and opt.state[p]["step"] == 1
+        opt.param_groups[0]["weight_decay"] = 0.3  # what a program sets from here on is AdamW's, and loads again
+        again = AdamW([torch.nn.Parameter(p.detach().clone())])
+        again.load_state_dict(opt.state_dict())
+        assert again.param_groups[0]["weight_decay"] == 0.3
