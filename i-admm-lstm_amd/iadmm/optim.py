@@ -154,6 +154,10 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError("a state with 32 bits does not load into an optimizer with 8")
             if s["exp_avg"].shape != p.shape or s["exp_avg_sq"].shape != p.shape:
                 raise ValueError(f"a state of {tuple(s['exp_avg'].shape)} does not fit a parameter of {tuple(p.shape)}")
+            if "exponents" in s and ([s[k].dtype for k in ("exp_avg", "exp_avg_sq", "exponents")] !=
+                                     [torch.uint8, torch.uint8, torch.int8]
+                                     or s["exponents"].numel() != -(-p.numel() // ops.ADAM_BLOCK) * 2):
+                raise ValueError("not the codes and exponents of 8-bit moments (another optimizer may have cast them)")
         super().load_state_dict(state_dict)
         self._counts = {}
         for g in self.param_groups:  # (Adam's mark: without a decay it loads, and the group is AdamW's from here on)

@@ -69,3 +69,19 @@ def test_a_decay_inside_the_gradient_does_not_become_a_decoupled_one():
         again = AdamW([torch.nn.Parameter(p.detach().clone())])
         again.load_state_dict(opt.state_dict())
         assert again.param_groups[0]["weight_decay"] == 0.3
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_codes_that_are_none_are_refused_before_anything_is_loaded(bits):
+    def state(codes=torch.uint8, exps=torch.int8, blocks=2):
+        one = dict(step=3, exp_avg=torch.zeros(300, dtype=codes), exp_avg_sq=torch.zeros(300, dtype=codes),
+                   exponents=torch.zeros(blocks, 2, dtype=exps))
+        return dict(state={0: one}, param_groups=[dict(opt.param_groups[0], params=[0], lr=0.5)])
+    opt = AdamW([parameter(300)], state_bits=bits)
+    for kw in (dict(codes=torch.float32), dict(exps=torch.float32), dict(blocks=1), dict(blocks=3)):
+        with pytest.raises(ValueError, match="8-bit moments"):
+            opt.load_state_dict(state(**kw))
+        assert not opt.state and opt.param_groups[0]["lr"] == 1e-3
+    if bits == 8:
+        opt.load_state_dict(state())
+        assert opt.state[opt.param_groups[0]["params"][0]]["exponents"].shape == (2, 2)
