@@ -63,7 +63,7 @@ def build_parser():
     add("--state_bits", type=int, choices=(8, 32), default=32, help="train: bits of AdamW's moments")
     add("--max_grad_norm", type=float, default=0.0, help="train: clip AdamW's gradients by their global norm (0: off)")
     add("--layer_norm", action="store_true", help="a model that normalises the hidden state before the gates' product")
-    add("--resume", type=str, default="", help="train: state file (model, Adam, epoch, EarlyStopping) written after "
+    add("--resume", type=str, default="", help="train: state file (model, optimizer, epoch, EarlyStopping) written after "
                                                "every epoch and continued from when it exists")
     return p
 
@@ -344,6 +344,25 @@ def report_stats(d, x, mi, me, dist):
     return out
 
 
+def optimizer_kind(optimizer):
+    """(--optimizer, --state_bits) of a make_optimizer result."""
+    return ("adamw", optimizer.state_bits) if hasattr(optimizer, "state_bits") else ("adam", 32)
+
+
+def check_resumed_optimizer(path, st, optimizer):
+    """Ends the run where another optimizer wrote the --resume state: torch's Adam would take 8-bit codes, cast to fp32, for
+    its moments.  A state without the entry goes by what only one of them writes: exponents, or no amsgrad."""
+    kind = st.get("optimizer_kind")
+    if kind is None:
+        saved = st["optimizer"]
+        if any("exponents" in s for s in saved["state"].values()):
+            kind = ("adamw", 8)
+        elif "amsgrad" not in saved["param_groups"][0]:
+            kind = ("adamw", 32)
+    if kind is not None and tuple(kind) != optimizer_kind(optimizer):
+        raise SystemExit(f"{path} was written by a run with --optimizer {kind[0]} --state_bits {kind[1]}: resume it with these")
+
+
 def save_resume_state(path, model, optimizer, epoch, stopper):
     """The --resume state file: tensors and plain Python scalars only, so that
     torch.load(weights_only=True) reads it back (EarlyStopping's best_loss becomes an np.float64
@@ -351,7 +370,8 @@ def save_resume_state(path, model, optimizer, epoch, stopper):
     to a temporary file and renamed into place, so a run killed mid-write keeps the previous state."""
     best = stopper.best_loss
     state = {"model": model.state_dict(), "optimizer": optimizer.state_dict(), "epoch": int(epoch),
-             "best_loss": None if best is None else float(best), "counter": int(stopper.counter)}
+             "best_loss": None if best is None else float(best), "counter": int(stopper.counter),
+             "optimizer_kind": list(optimizer_kind(optimizer))}
     tmp = path + ".tmp"
     torch.save(state, tmp)
     os.replace(tmp, path)
@@ -384,6 +404,7 @@ def run_train(args):
     first_epoch = 0
     if args.resume and os.path.exists(args.resume):  # this repo's own state file (tensors + scalars only)
         st = torch.load(args.resume, map_location=device, weights_only=True)
+        check_resumed_optimizer(args.resume, st, optimizer)
         model.load_state_dict(st["model"])
         optimizer.load_state_dict(st["optimizer"])
         stopper.best_loss, stopper.counter = st["best_loss"], int(st["counter"])

@@ -85,3 +85,36 @@ def test_codes_that_are_none_are_refused_before_anything_is_loaded(bits):
     if bits == 8:
         opt.load_state_dict(state())
         assert opt.state[opt.param_groups[0]["params"][0]]["exponents"].shape == (2, 2)
+
+
+def optimizer_of(kind, bits):
+    """main.make_optimizer's, with a state as after one step."""
+    import main
+    args = main.parse_args(["--lr", "0.1", "--optimizer", kind, "--state_bits", str(bits)])
+    opt = main.make_optimizer(args, [parameter()])
+    p = opt.param_groups[0]["params"][0]
+    if kind == "adamw":
+        opt._state(p)["step"] = 1
+    else:
+        p.grad = torch.ones(3)
+        opt.step()
+    return opt
+
+
+@pytest.mark.parametrize("older", [False, True])
+@pytest.mark.parametrize("wrote", [("adam", 32), ("adamw", 32), ("adamw", 8)])
+@pytest.mark.parametrize("reads", [("adam", 32), ("adamw", 32), ("adamw", 8)])
+def test_resume_goes_on_with_the_optimizer_that_wrote_the_state(wrote, reads, older, tmp_path):
+    """``older``: a file from before the optimizer was named in it, where Adam's entries alone tell nothing."""
+    import main
+    from utils import EarlyStopping
+    path = str(tmp_path / "resume.pt")
+    main.save_resume_state(path, torch.nn.Linear(1, 1), optimizer_of(*wrote), 0, EarlyStopping(str(tmp_path / "m.pth")))
+    st = torch.load(path, weights_only=True)
+    if older:
+        del st["optimizer_kind"]
+    if wrote == reads or (older and wrote[0] == "adam"):
+        main.check_resumed_optimizer(path, st, optimizer_of(*reads))
+    else:
+        with pytest.raises(SystemExit, match=f"--optimizer {wrote[0]} --state_bits {wrote[1]}"):
+            main.check_resumed_optimizer(path, st, optimizer_of(*reads))
