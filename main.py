@@ -135,6 +135,24 @@ def checkpoint_path(args, model_name="lstm"):
     return os.path.join(args.save_dir, model_name, "params", name)
 
 
+def train_path(args, model_name="lstm"):
+    """The weights file of a training run (main.py:88-92)."""
+    return os.path.join(args.save_dir, model_name, "params", "QP_{}_{}_{}_{}_{}.pth".format(
+        args.num_var, args.num_ineq, args.num_eq, args.outer_T, args.hidden_dim))
+
+
+def check_weights_kind(path, layer_norm):
+    """Ends the run where ``path`` holds the weights of the other kind of model: the reference's file names do not tell a
+    model with --layer_norm from one without, and training would write over them.  A file that does not load is nobody's."""
+    try:
+        saved = torch.load(path, map_location="cpu", weights_only=True)
+    except Exception:
+        return
+    if isinstance(saved, dict) and ("ln_w" in saved) != bool(layer_norm):
+        raise SystemExit(f"{path} holds a model {'without' if layer_norm else 'with'} --layer_norm: "
+                         "use another --save_dir, or the same option")
+
+
 def run_test(args):
     from models.lstm import LSTM
     if args.prob_type not in dataset.LAYOUTS or (args.synthetic and args.prob_type != "QP"):
@@ -152,6 +170,7 @@ def run_test(args):
     model = LSTM(mi + me, args.input_dim, args.hidden_dim, args.outer_T, device, layer_norm=args.layer_norm)
     ck = checkpoint_path(args, model.name())
     if os.path.exists(ck):
+        check_weights_kind(ck, args.layer_norm)
         model.load_state_dict(torch.load(ck, map_location=device, weights_only=True))
     elif not args.random_init:
         raise SystemExit(f"no checkpoint at {ck} (pass --random_init to run with random weights)")
@@ -384,6 +403,7 @@ def run_train(args):
     from utils import EarlyStopping
     if args.prob_type != "QP":
         raise SystemExit(f"prob_type {args.prob_type!r} is out of scope (DESIGN.md §0); use QP")
+    check_weights_kind(train_path(args), args.layer_norm)
     world, rank, local = parallel.env()
     device = f"cuda:{local}" if world > 1 else (args.device or "cuda:0")
     torch.cuda.set_device(torch.device(device))
@@ -391,8 +411,7 @@ def run_train(args):
     mi, me = args.num_ineq, args.num_eq
     torch.manual_seed(args.seed)
     model = LSTM(mi + me, args.input_dim, args.hidden_dim, args.outer_T, device, layer_norm=args.layer_norm)
-    save_path = os.path.join(args.save_dir, model.name(), "params", "QP_{}_{}_{}_{}_{}.pth".format(
-        args.num_var, args.num_ineq, args.num_eq, args.outer_T, args.hidden_dim))  # main.py:88-92
+    save_path = train_path(args, model.name())
     if rank == 0:
         os.makedirs(os.path.dirname(save_path), exist_ok=True)
     stopper = EarlyStopping(save_path, patience=args.patience)

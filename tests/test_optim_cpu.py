@@ -118,3 +118,31 @@ def test_resume_goes_on_with_the_optimizer_that_wrote_the_state(wrote, reads, ol
     else:
         with pytest.raises(SystemExit, match=f"--optimizer {wrote[0]} --state_bits {wrote[1]}"):
             main.check_resumed_optimizer(path, st, optimizer_of(*reads))
+
+
+def weights_file(path, layer_norm):
+    from models.lstm import LSTM
+    path.parent.mkdir(parents=True, exist_ok=True)
+    torch.save(LSTM(4, 2, 8, 3, "cpu", layer_norm=layer_norm).state_dict(), path)
+
+
+@pytest.mark.parametrize("held", [False, True])
+def test_weights_of_the_other_kind_of_model_are_not_written_over(held, tmp_path):
+    """The file names are the reference's for both kinds: the run ends before it touches a device or the file."""
+    import main
+    argv = ["--prob_type", "QP", "--num_var", "5", "--num_ineq", "3", "--num_eq", "1", "--outer_T", "3", "--hidden_dim", "8",
+            "--lr", "0.1", "--synthetic", "--save_dir", str(tmp_path)]
+    other = [] if held else ["--layer_norm"]
+    path = tmp_path / "lstm" / "params" / "QP_5_3_1_3_8.pth"
+    weights_file(path, held)
+    before = path.read_bytes()
+    with pytest.raises(SystemExit, match="without --layer_norm" if not held else "with --layer_norm"):
+        main.main(argv + other)
+    assert path.read_bytes() == before
+    args = main.parse_args(argv)
+    assert main.train_path(args) == str(path)
+    main.check_weights_kind(str(path), held)                      # its own kind goes on over it
+    for kind in (False, True):
+        main.check_weights_kind(str(tmp_path / "none.pth"), kind)
+        (tmp_path / "cut.pth").write_bytes(before[:100])          # what an interrupted run left
+        main.check_weights_kind(str(tmp_path / "cut.pth"), kind)
