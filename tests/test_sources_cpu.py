@@ -1,6 +1,8 @@
 """What the sources that reach the GPU may not hold, read as text (no GPU)."""
 import glob
 import os
+import re
+import subprocess
 
 REPO = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 PKG = os.path.join(REPO, "i-admm-lstm_amd")
@@ -20,3 +22,30 @@ def test_every_stream_has_the_default_priority():
         with open(path) as f:
             text = f.read()
         assert "hipStreamCreateWithPriority" not in text, path
+
+
+def test_every_build_leaves_packed_fp32_out():
+    """Some forms of v_pk_add / mul / fma_f32 have given wrong results on this hardware: the flag is in the library's build,
+    in a variant's (the same Makefile, told another place) and in the command that a tool's source names; none is written by hand."""
+    off = "-Xclang -target-feature -Xclang -packed-fp32-ops"
+    lines = subprocess.run(["make", "-n", "-B", "-C", PKG, "all"], capture_output=True, text=True, check=True).stdout.splitlines()
+    compiled = [line for line in lines if "hipcc" in line and " -c " in line]
+    assert len(compiled) >= 12 and all(off in line for line in compiled)
+    with open(os.path.join(REPO, "tools", "build_variant.sh")) as f:
+        script = f.read()
+    assert "hipcc" not in script and "make" in script
+    for path in hip_sources() + glob.glob(os.path.join(REPO, "tools", "*.py")) + glob.glob(os.path.join(REPO, "tools", "*.sh")):
+        with open(path) as f:
+            text = f.read()
+        assert not re.search(r'"[^"\n]*v_pk_(add|mul|fma)_f32 ', text), path
+        for m in re.finditer(r"hipcc\b[^\n]*--offload-arch", text):
+            assert "-packed-fp32-ops" in text[m.start():m.start() + 200], f"{path}: {m.group()}"
+
+
+def test_a_variant_has_every_source_of_the_library(tmp_path):
+    lines = subprocess.run(["make", "-n", "-C", PKG, f"CSRC={PKG}/csrc", f"BLD={tmp_path}/o", f"OUT={tmp_path}/v.so",
+                            "EXTRA=-DNAME=1", f"{tmp_path}/v.so"], capture_output=True, text=True, check=True).stdout
+    own = {os.path.basename(f) for f in glob.glob(os.path.join(PKG, "csrc", "*.hip"))}
+    compiled = re.findall(r"-DNAME=1 -c \S*/csrc/(\w+\.hip) ", lines)
+    assert set(compiled) == own and len(compiled) == len(own)
+    assert f"-o {tmp_path}/v.so" in lines

@@ -2,7 +2,7 @@
 // Descriptor over the first 256 B of a 4 KiB zeroed buffer; lane 0 stores 1.0 with voffset 0 and
 // soffset 512 (in range without soffset, out of range with it); lane 1 voffset 512, soffset 0
 // (out of range either way).  Prints what landed at bytes 512 and 516.
-// Build: hipcc -O3 --offload-arch=gfx950 tools/buffer_soffset_probe.hip -o tools/buffer_soffset_probe.bin
+// Build: hipcc -O3 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops tools/buffer_soffset_probe.hip -o tools/buffer_soffset_probe.bin
 #include <hip/hip_runtime.h>
 #include <cstdio>
 __global__ void probe(float* p, int so) {

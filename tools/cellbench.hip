@@ -1,7 +1,7 @@
 // Variant microbenchmark of the fused LSTM-cell kernel at the bench shape (M = 1024*2000 rows,
 // h = 800): interleaved rounds of every variant in one process (cdna_hip_programming.md §5.4
 // rule 24), hipEvent timing, TFLOP/s on the algorithmic 8*M*h^2 + 18*M*h flops.
-// Build: hipcc -O3 -std=c++17 --offload-arch=gfx950 -ffp-contract=off -mllvm -disable-promote-alloca-to-lds \
+// Build: hipcc -O3 -std=c++17 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -ffp-contract=off -mllvm -disable-promote-alloca-to-lds \
 //          tools/cellbench.hip -o tools/cellbench.bin
 // Variants are instances of the production kernel template (cell_tile.h cell_fwd_kernel<VEC, NW,
 // PRIO>); the first is the one lstm.hip launches.  Round-1 study of earlier variants (BK 16 / double

@@ -1,7 +1,7 @@
 """Co-residency probe: does an HBM-streaming kernel run beside the cell kernel without taking its
 CU slots?  (overlap of the residual matvec with the cell kernel.)
 
-  python tools/costream.py            (needs tools/costream.so: hipcc --offload-arch=gfx950 -O3
+  python tools/costream.py            (needs tools/costream.so: hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3
                                         -shared -fPIC tools/costream.hip -o tools/costream.so)
 
 Times, on one GPU: the cell kernel of B instances alone; a lean one-wave streaming reader alone;

@@ -2,7 +2,7 @@
 // bench shape (B = 1024, N = 2000), first block (K0 = 0, 1936 x 1936 trailing matrix):
 // hipEvent timing of the kernel and of its memory pipeline alone (DIAG 1: no MFMAs), algorithmic GB/s
 // on the A22 read + write.
-// Build: hipcc -O3 -std=c++17 --offload-arch=gfx950 tools/lubench.hip -o tools/lubench.bin
+// Build: hipcc -O3 -std=c++17 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops tools/lubench.hip -o tools/lubench.bin
 #include "../i-admm-lstm_amd/csrc/lu.hip"
 
 #include <cstdio>

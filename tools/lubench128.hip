@@ -7,7 +7,7 @@
 // interchanges are exercised by the Stage-II tests, not here.)
 // Earlier variants: the r04 wave-specialised kernel (4 MFMA + 8 memory waves; bitwise equal, 6 %
 // slower, profiles/r04_lubench128_ws_rejected.txt) is in this file's history.
-// Build: hipcc -O3 -std=c++17 --offload-arch=gfx950 tools/lubench128.hip -o tools/lubench128.bin
+// Build: hipcc -O3 -std=c++17 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops tools/lubench128.hip -o tools/lubench128.bin
 #include "../i-admm-lstm_amd/csrc/lu.hip"
 
 #include <cstdio>

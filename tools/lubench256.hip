@@ -6,7 +6,7 @@
 // exercised, through the identity tables).  Results of the diagnostic variants are meaningless (and
 // no-mem ones are void: the compiler drops the chain whose result is never stored).
 // (r05 second form, one 8-wave workgroup per CU: profiles/r05_lubench256.txt, in this file's history.)
-// Build: hipcc -O3 -std=c++17 --offload-arch=gfx950 tools/lubench256.hip -o tools/lubench256.bin
+// Build: hipcc -O3 -std=c++17 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops tools/lubench256.hip -o tools/lubench256.bin
 #include "../i-admm-lstm_amd/csrc/lu.hip"
 
 #include <cstdio>

@@ -3,7 +3,7 @@
 // without its column steps (DIAG 1), without panel_finish (the in-block interchanges and the
 // 16-row TRSM; DIAG 2), and with neither (the panel's load and store alone; DIAG 3).  hipEvents,
 // median of 5 launches each, on the same (refactored in place) matrices.
-// Build: hipcc -O3 -std=c++17 --offload-arch=gfx950 tools/lupanelbench.hip -o tools/lupanelbench.bin
+// Build: hipcc -O3 -std=c++17 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops tools/lupanelbench.hip -o tools/lupanelbench.bin
 #include "../i-admm-lstm_amd/csrc/lu.hip"
 
 #include <algorithm>

@@ -1,7 +1,7 @@
 // Accuracy of the LSTM-cell transcendentals (common.h sigmoid_cell / tanh_cell) against fp64, next
 // to the libm-accurate forms (sigmoidf_ / tanhf): max and mean error in fp32 ulps of the exact
 // result, max absolute error, max relative error where |f| > 1e-3, over every fp32 value in
-// [-30, 30] with a stride (plus all of [-1, 1] at a finer stride); tails: absolute error <= 5e-7.  Build: hipcc -O3 --offload-arch=gfx950 -ffp-contract=off tools/mathcheck.hip -o tools/mathcheck.bin
+// [-30, 30] with a stride (plus all of [-1, 1] at a finer stride); tails: absolute error <= 5e-7.  Build: hipcc -O3 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -ffp-contract=off tools/mathcheck.hip -o tools/mathcheck.bin
 #include "../i-admm-lstm_amd/csrc/common.h"
 #include <cstdio>
 #include <cmath>

@@ -1,7 +1,7 @@
 // Issue rate of v_mfma_f32_32x32x2f32 chains on gfx950: NACC independent accumulators per wave
 // (NACC = 1: every MFMA depends on the previous one through its accumulator, as in the LU trailing
 // update's per-wave 32x32 tile), 1 or 2 waves per SIMD (WPS).  Prints cycles per MFMA per SIMD.
-// Build: hipcc -O3 -std=c++17 --offload-arch=gfx950 tools/mfma_chain_probe.hip -o tools/mfma_chain_probe.bin
+// Build: hipcc -O3 -std=c++17 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops tools/mfma_chain_probe.hip -o tools/mfma_chain_probe.bin
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdlib>

@@ -1,7 +1,7 @@
 // Does v_mfma_f32_32x32x2_f32 round each product before accumulating (unlike an FMA)?  acc =
 // -(1 + 2^-22) + (1 + 2^-23)^2: an exact (fused) product leaves 2^-46, a rounded product 0.  Also the
 // same with the product in the second k slot, and the VALU fmaf for comparison.
-// Build: hipcc -O3 --offload-arch=gfx950 tools/mfma_fma_check.hip -o tools/mfma_fma_check.bin
+// Build: hipcc -O3 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops tools/mfma_fma_check.hip -o tools/mfma_fma_check.bin
 #include <hip/hip_runtime.h>
 #include <cstdio>
 
