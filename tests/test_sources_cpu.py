@@ -49,3 +49,11 @@ def test_a_variant_has_every_source_of_the_library(tmp_path):
     compiled = re.findall(r"-DNAME=1 -c \S*/csrc/(\w+\.hip) ", lines)
     assert set(compiled) == own and len(compiled) == len(own)
     assert f"-o {tmp_path}/v.so" in lines
+
+
+def test_build_compiles_what_is_built_already(monkeypatch):
+    import __graft_entry__ as entry
+    ran = []
+    monkeypatch.setattr(entry.subprocess, "run", lambda cmd, **kw: ran.append(cmd))
+    entry.build()
+    assert len(ran) == 1 and ran[0][0] == "make" and "-B" in ran[0]
