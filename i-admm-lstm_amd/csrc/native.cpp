@@ -65,6 +65,12 @@ bool has_rows(const Tensor& t) {
   return t.is_contiguous() || (t.dim() == 2 && t.stride(1) == 1 && t.stride(0) >= t.size(1));
 }
 
+// The tensor, or a copy where its rows are not contiguous or torch negates it on reading.
+Tensor plain_rows(const Tensor& t) {
+  const Tensor p = t.is_neg() ? t.resolve_neg() : t;
+  return has_rows(p) ? p : p.contiguous();
+}
+
 struct Rows { int64_t rows, cols, ld; };
 
 Rows rows_of(const Tensor& t, const char* what) {
@@ -184,7 +190,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &w = saved[1];
     if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
-    const Tensor dy = has_rows(grads[0]) ? grads[0] : grads[0].contiguous();  // (a sum's gradient is expanded)
+    const Tensor dy = plain_rows(grads[0]);  // (a sum's gradient is expanded)
     std::vector<Tensor> out;
     {
       const at::AutoGradMode off(false);
@@ -329,7 +335,7 @@ PyObject* py_layer_norm_grad(PyObject*, PyObject* const* a, Py_ssize_t n) {
   TORCH_CHECK_VALUE(x.layout() == at::kStrided, "x must be a dense tensor");
   const std::optional<Tensor> weight = w.defined() ? std::optional(w) : std::nullopt,
                               bias = b.defined() ? std::optional(b) : std::nullopt;  // (edges only for those that are)
-  return wrap(LayerNorm::apply(has_rows(x) ? x : x.contiguous(), weight, bias, eps));
+  return wrap(LayerNorm::apply(plain_rows(x), weight, bias, eps));
   END_HANDLE_TH_ERRORS
 }
 

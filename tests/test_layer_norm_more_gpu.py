@@ -1,0 +1,47 @@
+"""autograd.layer_norm as part of a program: views that torch negates on reading, checkpoints, hooks on saved tensors,
+transforms that it refuses, captured graphs, long columns."""
+import pytest
+import torch
+
+import iadmm_path  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+@pytest.fixture(autouse=True)
+def _gpu():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+
+
+def inputs(rows, cols, t=F32, seed=0):
+    """x, dy, weight, bias; the first and the last two leaves."""
+    g = torch.Generator().manual_seed(seed * 1000003 + rows * 1009 + cols)
+    r = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    x, dy = ((r(rows, cols) + 0.3).to(t).cuda() for _ in range(2))
+    w, b = (1 + 0.3 * r(cols)).cuda(), (0.2 * r(cols)).cuda()
+    return x.requires_grad_(), dy, w.requires_grad_(), b.requires_grad_()
+
+
+def gradients(x, w, b, dy, run=None):
+    from iadmm import autograd
+    y = (run or autograd.layer_norm)(x, w, b)
+    return [y.detach(), *torch.autograd.grad(y, (x, w, b), dy)]
+
+
+def same(got, want):
+    return all(torch.equal(a, c) for a, c in zip(got, want))
+
+
+def test_negated_views():
+    """As an input and as the gradient that arrives: the bits of their negated copies."""
+    from iadmm import autograd
+    x, dy, w, b = inputs(9, 65)
+    want = gradients((-x).detach().requires_grad_(), w, b, -dy)
+    y = autograd.layer_norm(torch._neg_view(x), w, b)
+    got = torch.autograd.grad(y, (x, w, b), torch._neg_view(dy), retain_graph=True)
+    assert torch.equal(y, want[0]) and torch.equal(got[0], -want[1]) and same(got[1:], want[2:])
+    y.register_hook(lambda g: torch._neg_view(g))
+    assert same(torch.autograd.grad(y, (x, w, b), dy), got)
