@@ -98,7 +98,8 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        grads = [[None if p.grad is None else p.grad.contiguous() for p in g["params"]] for g in self.param_groups]
+        plain = lambda x: (x.resolve_neg() if x.is_neg() else x).contiguous()  # noqa: E731
+        grads = [[None if p.grad is None else plain(p.grad) for p in g["params"]] for g in self.param_groups]
         every = [x for gs in grads for x in gs if x is not None]
         if not every:
             return loss

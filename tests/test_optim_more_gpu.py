@@ -74,3 +74,15 @@ def test_counts_follow_the_parameters_not_their_place():
         ends.append([p.detach().clone() for p in a[:2]])
     for p, q in zip(*ends):  # (the corrections of the two kinds of counts are rounded apart: 2 u of an update, 7 updates)
         assert bool(((p - q).abs() <= 7 * 2.0 ** -24 * (4 * p.abs() + 24 * 2e-2)).all())
+
+
+def test_gradients_that_are_negated_views():
+    from iadmm.optim import AdamW
+    a, b = params(), params()
+    set_grads(a, 0)
+    for p, q in zip(a, b):
+        q.grad = torch._neg_view(-p.grad)
+    one, two = AdamW(a, max_norm=1.0), AdamW(b, max_norm=1.0)
+    one.step()
+    two.step()
+    assert torch.equal(one.norm, two.norm) and all(torch.equal(p, q) for p, q in zip(a, b))
