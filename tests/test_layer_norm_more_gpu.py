@@ -45,3 +45,44 @@ def test_negated_views():
     assert torch.equal(y, want[0]) and torch.equal(got[0], -want[1]) and same(got[1:], want[2:])
     y.register_hook(lambda g: torch._neg_view(g))
     assert same(torch.autograd.grad(y, (x, w, b), dy), got)
+
+
+def test_captured_backward_pass():
+    """Replays, with eager passes over leaves of their own between them, give the eager bits.  A capture beside a graph of
+    the same leaves that is still alive is refused, and leaves that graph usable."""
+    from iadmm import autograd
+    x, dy, w, b = inputs(333, 800)
+    leaves = (x, w, b)
+
+    def captured():
+        for t in leaves:
+            t.grad = None
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = autograd.layer_norm(x, w, b)
+            y.backward(dy)
+        return g, y.detach()
+
+    alive = autograd.layer_norm(x, w, b)
+    for t in leaves:
+        t.grad = None
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        with pytest.raises(RuntimeError, match="still alive"):
+            autograd.layer_norm(x, w, b).backward(dy)
+        with pytest.raises(RuntimeError, match="still alive"):
+            torch.autograd.grad(autograd.layer_norm(x, w, b), (w,), dy)
+    assert all(t.grad is None for t in leaves)
+    assert same(torch.autograd.grad(alive, leaves, dy), gradients(x, w, b, dy)[1:])
+    del alive
+    torch.cuda.synchronize()
+    graph, y = captured()
+    grads = [t.grad for t in leaves]
+    for k in range(4):
+        x2, dy2, w2, b2 = inputs(333, 800, seed=k + 1)
+        with torch.no_grad():
+            for t, s in ((x, x2), (dy, dy2), (w, w2), (b, b2)):
+                t.copy_(s)
+        want = gradients(x2, w2, b2, dy2)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert same([y, *grads], want), k
