@@ -448,7 +448,10 @@ PyObject* py_adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!counted && !numbers) step = PyLong_AsLongLong(a[5]);
   std::vector<iadmm_adamw_tensor> rec(use.size());
   std::vector<Held> held;
-  held.reserve(use.size() * 5);
+  held.reserve(use.size() * 5 + 3);
+  if (counted) held.emplace_back(counts.const_data_ptr(), count * static_cast<int64_t>(sizeof(int64_t)), true);
+  for (const Tensor* t : {&lr_dev, &norm})
+    if (t->defined()) held.emplace_back(t->const_data_ptr(), 4, false);
   for (size_t k = 0; k < use.size(); ++k) {
     const int64_t size = p.t[k].numel();
     TORCH_CHECK_VALUE(g.t[k].sizes() == p.t[k].sizes(), "gradient ", use[k], " is ", g.t[k].sizes(), ", its parameter ",

@@ -86,3 +86,23 @@ def test_gradients_that_are_negated_views():
     one.step()
     two.step()
     assert torch.equal(one.norm, two.norm) and all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def test_numbers_on_the_device_that_lie_in_what_is_written_are_refused():
+    """norm, lr and the steps' counts: every workgroup reads the first two while others write, and writes the third once."""
+    from iadmm import ops
+    buf = torch.rand(1000, device="cuda") + 0.5
+    keep = buf.clone()
+    p, g, m, v = buf[:300], torch.randn(300, device="cuda"), buf[300:600], buf[600:900]
+    counts = torch.zeros(1, dtype=torch.int64, device="cuda")
+    inside = buf[298:300].view(torch.int64)
+    for kw in (dict(step=1, norm=p[7], max_norm=1.0), dict(step=1, norm=m[299], max_norm=1.0), dict(step=counts, lr=v[:1]),
+               dict(step=inside), dict(step=counts, lr=counts.view(torch.float32)[1:]),
+               dict(step=counts, norm=counts.view(torch.float32)[0], max_norm=1.0)):
+        with pytest.raises(ValueError, match="overlaps"):
+            ops.adamw_step([p], [g], [m], [v], **kw)
+    torch.cuda.synchronize()
+    assert torch.equal(buf, keep) and int(counts) == 0
+    ops.adamw_step([p], [g], [m], [v], counts, lr=buf[900:901], norm=g[5].abs(), max_norm=1.0)  # side by side
+    ops.adamw_step([p], [g], [m], [v], 2, norm=g[5:6], max_norm=1.0)                            # a gradient is only read
+    assert int(counts) == 1 and torch.equal(buf[900:], keep[900:]) and not torch.equal(p, keep[:300])
