@@ -561,6 +561,10 @@ def layer_norm_bwd(dy, x, mean, rstd, weight=None, need=(True, True, True), wdty
     dx has x's type, dweight and dbias weight's (``wdtype`` or fp32 without a weight).  ``need``: which to
     compute (the others are None).  The sums over rows have a fixed order: the same inputs give the same
     bits."""
+    if wdtype is not None and wdtype not in DTYPES:
+        raise TypeError(f"wdtype must be float32, bfloat16 or float16, got {wdtype}")
+    if len(need) != 3:
+        raise ValueError(f"need must say of dx, dweight and dbias whether to compute them, got {need}")
     return _abi.native().layer_norm_bwd(dy, x, mean, rstd, weight, DTYPES[wdtype or torch.float32], *need)
 
 
