@@ -86,3 +86,26 @@ def test_captured_backward_pass():
         graph.replay()
         torch.cuda.synchronize()
         assert same([y, *grads], want), k
+
+
+@pytest.mark.parametrize("t", [F32, BF16])
+def test_many_long_rows(t):
+    """A column of a few thousand rows has at most 48 + rows / 32 roundings of u = 2^-24 in its sums also where a row is so long that
+    only two workgroups share a column.  dy repeats one number in each column, chosen so that a chain in fp32 rounds
+    the same way each time: half a thousand times by 0.45 of a last place in the sum's last binade (208 roundings in all);
+    in bf16 it is exact."""
+    from iadmm import ops
+    rows, cols = 2048, 524291 if t == F32 else 2 * 524291
+    value = 1 + 0.9 * 2.0 ** -15 if t == F32 else 1 + 2.0 ** -7
+    x = torch.empty(rows, cols, dtype=t, device="cuda").normal_(generator=torch.Generator(device="cuda").manual_seed(3))
+    dy = torch.full((rows, cols), value, dtype=t, device="cuda")
+    _, mean, rstd = ops.layer_norm(x, stats=True)
+    _, dw, db = ops.layer_norm_bwd(dy, x, mean, rstd, need=(False, True, True))
+    u, roundings = 2.0 ** -24, 48 + rows / 32
+    want = rows * float(dy[0, 0])
+    assert float((db.double() - want).abs().max()) <= (roundings + 1) * u * want
+    for c in range(0, cols, 65536):
+        part = slice(c, min(c + 65536, cols))
+        terms = (x[:, part].double() - mean.double()[:, None]) * rstd.double()[:, None] * float(dy[0, 0])
+        off = (dw[part].double() - terms.sum(0)).abs()
+        assert bool((off <= roundings * u * terms.abs().sum(0) + u * terms.sum(0).abs()).all()), c
