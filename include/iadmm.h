@@ -128,8 +128,9 @@ int iadmm_kkt_rhs(int64_t B, int64_t n, int64_t m, int64_t num_ineq, const float
  * factors the next block beside the rest of each trailing update (look-ahead) on the context's two
  * streams, forked from and joined back into `stream` on every path, errors
  * included: the call stays asynchronous and ordered on `stream`, and the factors are bit for bit
- * those of iadmm_lu_factor.  Under stream capture (hipGraph) the call ignores the context and runs
- * every launch on `stream` (the cross-stream fork / join crashed the HIP 7.2 runtime at capture end).
+ * those of iadmm_lu_factor.  Under stream capture (hipGraph) the side work forks from `stream` itself, so that
+ * the captured graph has the same concurrency (a fork from a stream that joined the capture through another
+ * fork crashes PyTorch's bundled HIP 7.0.2 runtime at capture end).
  * A context belongs to the device current at its creation (IADMM_E_ARG on another) and serves one
  * factorization at a time in its streams' order: give each concurrent caller (thread / stream) its own.
  * Block pairs (r05, the default for N <= 2048 with N % 4 == 0 and 16-B aligned rows): two 128-column
