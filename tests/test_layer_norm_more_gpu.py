@@ -109,3 +109,46 @@ def test_many_long_rows(t):
         terms = (x[:, part].double() - mean.double()[:, None]) * rstd.double()[:, None] * float(dy[0, 0])
         off = (dw[part].double() - terms.sum(0)).abs()
         assert bool((off <= roundings * u * terms.abs().sum(0) + u * terms.sum(0).abs()).all()), c
+
+
+@pytest.mark.parametrize("t", [F32, F16])
+def test_checkpoints_and_hooks_on_saved_tensors(t):
+    """What is saved may be made again or lie elsewhere until the backward pass: the same bits."""
+    from torch.utils.checkpoint import checkpoint
+    from iadmm import autograd
+    x, dy, w, b = inputs(70, 801, t)
+    want = gradients(x, w, b, dy)
+    for reentrant in (False, True):
+        for p in (x, w, b):
+            p.grad = None
+        y = checkpoint(autograd.layer_norm, x, w, b, use_reentrant=reentrant)
+        y.backward(dy)
+        assert same([y.detach(), x.grad, w.grad, b.grad], want)
+    with torch.autograd.graph.save_on_cpu():
+        y = autograd.layer_norm(x, w, b)
+    assert same(torch.autograd.grad(y, (x, w, b), dy), want[1:])
+    seen = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda s: seen.append(s) or s.clone(), lambda s: s):
+        y = autograd.layer_norm(x, w, b)
+    assert same(torch.autograd.grad(y, (x, w, b), dy), want[1:]) and len(seen) == 4
+
+
+def test_transforms_are_refused():
+    """Batched, functional and forward-mode tensors: an error, nothing computed.  A compiled caller runs the call as it is."""
+    import torch.autograd.forward_ad as forward_ad
+    from iadmm import autograd, ops
+    x, dy, w, b = inputs(6, 40)
+    d = x.detach()
+    for call in (lambda: torch.func.vmap(lambda r: autograd.layer_norm(r))(d.view(2, 3, 40)),
+                 lambda: torch.func.vmap(lambda r: ops.layer_norm(r))(d.view(2, 3, 40)),
+                 lambda: torch.func.vmap(lambda v: ops.layer_norm(d, v))(w.detach().expand(3, 40).contiguous()),
+                 lambda: torch.func.grad(lambda s: autograd.layer_norm(s, w, b).sum())(d),
+                 lambda: torch.func.jvp(lambda s: autograd.layer_norm(s), (d,), (d,)),
+                 lambda: torch.autograd.functional.jacobian(autograd.layer_norm, d, vectorize=True)):
+        with pytest.raises(RuntimeError):
+            call()
+    with forward_ad.dual_level():
+        with pytest.raises(RuntimeError):
+            autograd.layer_norm(forward_ad.make_dual(d, dy), w, b)
+    y = torch.compile(lambda s: autograd.layer_norm(s + 0, w, b) + 0, backend="eager")(x)
+    assert same([y.detach(), *torch.autograd.grad(y, (x, w, b), dy)], gradients(x, w, b, dy))
