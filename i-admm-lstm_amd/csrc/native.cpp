@@ -52,6 +52,8 @@ void on_device(const Tensor& t, const char* what, const Tensor* like = nullptr) 
   TORCH_CHECK_VALUE(t.is_cuda(), "iadmm kernels need device tensors (no CPU fallback), and ", what, " is on ", t.device());
   TORCH_CHECK_VALUE(!like || t.device() == like->device(), what, " is on ", t.device(), ", not on ", like->device());
   TORCH_CHECK_VALUE(!t.is_neg(), what, " is a view that torch negates on reading: resolve_neg() it first");
+  // (a fake tensor of a tracing mode has none, and a null pointer would stand for an operand that is left out)
+  TORCH_CHECK_VALUE(t.layout() != at::kStrided || t.numel() == 0 || t.const_data_ptr(), what, " has no memory");
 }
 
 // A kernel wrote it behind autograd's back: whoever goes by its version (a graph that saved it, solver.PackedWeights) has
@@ -440,6 +442,8 @@ PyObject* py_adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
   for (const auto& [t, what] : {std::pair<const Tensor&, const char*>{lr_dev, "lr"}, {norm, "norm"}})
     TORCH_CHECK_VALUE(!t.defined() || (t.device() == p.device && t.scalar_type() == at::kFloat && t.numel() == 1), what,
                       " must be one float32 value on ", p.device);
+  for (const Tensor* t : {&lr_dev, &norm, &counts})
+    TORCH_CHECK_VALUE(!t->defined() || t->const_data_ptr(), "lr, norm or step has no memory");
   TORCH_CHECK_VALUE(!norm.defined() || most > 0.0, "max_norm must be positive, got ", most);
   TORCH_CHECK_VALUE(!counted || (counts.device() == p.device && counts.scalar_type() == at::kLong && counts.dim() == 1 &&
                                  counts.size(0) == count && counts.is_contiguous()),

@@ -152,3 +152,25 @@ def test_transforms_are_refused():
             autograd.layer_norm(forward_ad.make_dual(d, dy), w, b)
     y = torch.compile(lambda s: autograd.layer_norm(s + 0, w, b) + 0, backend="eager")(x)
     assert same([y.detach(), *torch.autograd.grad(y, (x, w, b), dy)], gradients(x, w, b, dy))
+
+
+def test_tensors_without_memory_are_refused():
+    """A fake tensor says that it is on the device and has no address: none may stand for an operand that is left out."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from iadmm import _abi, autograd, ops
+    x, dy, w, b = (p.detach() for p in inputs(6, 40))
+    mode = FakeTensorMode()
+    fx, fw, one = mode.from_tensor(x), mode.from_tensor(w), mode.from_tensor(w[:1].clone())
+    _, mean, rstd = ops.layer_norm(x, stats=True)
+    m, v = torch.zeros_like(x), torch.zeros_like(x)
+    keep = x.clone()
+    counts = torch.zeros(1, dtype=torch.int64, device="cuda")
+    for call in (lambda: ops.layer_norm(fx), lambda: ops.layer_norm(x, fw), lambda: ops.layer_norm(x, w, fw), lambda: autograd.layer_norm(x, fw),
+                 lambda: ops.layer_norm_bwd(dy, x, mean, rstd, fw), lambda: ops.layer_norm_bwd(fx, x, mean, rstd),
+                 lambda: ops.grad_norm([fx]), lambda: ops.adamw_step([x], [fx], [m], [v], 1),
+                 lambda: ops.adamw_step([x], [dy], [m], [v], 1, norm=one, max_norm=1.0),
+                 lambda: ops.adamw_step([x], [dy], [m], [v], counts, lr=one)):
+        with pytest.raises((RuntimeError, ValueError, _abi.IadmmError)):
+            call()
+    torch.cuda.synchronize()
+    assert torch.equal(x, keep) and int(counts) == 0
