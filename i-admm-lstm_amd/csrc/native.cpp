@@ -11,6 +11,7 @@
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
@@ -61,6 +62,9 @@ void on_device(const Tensor& t, const char* what, const Tensor* like = nullptr) 
 void written(const Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
+
+// A trace records torch's operations alone: the result would stand in it as a constant.
+void not_traced() { TORCH_CHECK(!torch::jit::tracer::isTracing(), "torch.jit.trace cannot record iadmm's kernels"); }
 
 Tensor f32_on(const Tensor& like, at::IntArrayRef shape) { return at::empty(shape, like.options().dtype(at::kFloat)); }
 
@@ -315,6 +319,7 @@ PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* py_layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   want(n, 6);
+  not_traced();
   TORCH_CHECK_TYPE(THPVariable_Check(a[0]), "x must be a tensor");
   const Tensor x = THPVariable_Unpack(a[0]), w = optional_tensor(a[1], "weight"), b = optional_tensor(a[2], "bias");
   const double eps = number(a[3]);
@@ -332,6 +337,7 @@ PyObject* py_layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* py_layer_norm_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   want(n, 9);
+  not_traced();
   for (int i = 0; i < 4; ++i) TORCH_CHECK_TYPE(THPVariable_Check(a[i]), "dy, x, mean and rstd must be tensors");
   const Tensor w = optional_tensor(a[4], "weight");
   const long half = PyLong_AsLong(a[5]);  // include/iadmm.h's type code
@@ -349,6 +355,7 @@ PyObject* py_layer_norm_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* py_layer_norm_grad(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   want(n, 4);
+  not_traced();
   TORCH_CHECK_TYPE(THPVariable_Check(a[0]), "x must be a tensor");
   const Tensor x = THPVariable_Unpack(a[0]), w = optional_tensor(a[1], "weight"), b = optional_tensor(a[2], "bias");
   const double eps = number(a[3]);
@@ -363,6 +370,7 @@ PyObject* py_layer_norm_grad(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* py_grad_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   want(n, 1);
+  not_traced();
   const Fast grads(a[0], "gradients must be a list");
   std::vector<int> use;
   for (int i = 0; i < grads.size(); ++i)
@@ -406,6 +414,7 @@ bool apart(std::vector<Held>& held) {
 PyObject* py_adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   want(n, 14);
+  not_traced();
   const Fast params(a[0], "params must be a list"), grads(a[1], "grads must be a list"),
       avgs(a[2], "exp_avgs must be a list"), sqs(a[3], "exp_avg_sqs must be a list");
   const bool eight = a[4] != Py_None, counted = THPVariable_Check(a[5]), numbers = !counted && !PyIndex_Check(a[5]);
