@@ -106,3 +106,56 @@ def test_numbers_on_the_device_that_lie_in_what_is_written_are_refused():
     ops.adamw_step([p], [g], [m], [v], counts, lr=buf[900:901], norm=g[5].abs(), max_norm=1.0)  # side by side
     ops.adamw_step([p], [g], [m], [v], 2, norm=g[5:6], max_norm=1.0)                            # a gradient is only read
     assert int(counts) == 1 and torch.equal(buf[900:], keep[900:]) and not torch.equal(p, keep[:300])
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_clipping_inside_a_training_window(bits):
+    """tbptt_batch's steps with a max_norm of half the gradients' norm: parameters and moments have the bits of an optimizer
+    without it that is given the gradients times the clipping factor, and no parameter moves by more than lr |m| / sqrt(v),
+    corrected: 1 at the first step; at the second m weighs the two gradients by (0.4737, 0.5263) and v their squares by
+    (0.49975, 0.50025), so at most sqrt(0.4737^2 / 0.49975 + 0.5263^2 / 0.50025) = 1.0014, with 24 roundings in all."""
+    from models.lstm import LSTM
+    from iadmm import data, ops, train
+    from iadmm.optim import AdamW
+
+    class Recorded(AdamW):
+        def step(self, closure=None):
+            ps = [p for g in self.param_groups for p in g["params"]]
+            grads = [None if p.grad is None else p.grad.clone() for p in ps]
+            out = super().step(closure)
+            self.seen.append((grads, self.norm.clone(), [p.detach().clone() for p in ps],
+                              [[m.clone() for m in self.moments(p)] for p in ps]))
+            return out
+
+    raw = data.make_qp_batch(40, 14, 6, 4, first_index=2, device="cuda")
+    d = dict(zip(("Q", "p", "A0", "zl", "zu"), ops.ruiz_scale(raw["Q"], raw["p"], raw["A0"], raw["zl"], raw["zu"], 10)[:5]))
+    T, lr = 6, 1e-3
+
+    def run(max_norm):
+        torch.manual_seed(3)
+        model = LSTM(20, 2, 48, T, "cuda", layer_norm=True)
+        start = [p.detach().clone() for p in model.parameters()]
+        opt = Recorded(model.parameters(), lr=lr, weight_decay=0.0, state_bits=bits, max_norm=max_norm, seed=9)
+        opt.seen = []
+        train.tbptt_batch(model, d, 14, 6, 2 * T, T, 6e-6, opt, micro_batch=2)
+        return start, opt.seen
+
+    _, free = run(1e9)
+    most = 0.5 * min(float(norm) for _, norm, _, _ in free)
+    start, seen = run(most)
+    assert len(seen) == len(free) == 2
+    own = [torch.nn.Parameter(p.clone()) for p in start]
+    plain = AdamW(own, lr=lr, weight_decay=0.0, state_bits=bits, seed=9)
+    before = start
+    for k, (grads, norm, after, moments) in enumerate(seen):
+        assert float(norm) > 1.5 * most
+        factor = torch.tensor(most, device="cuda") / (norm + 1e-6)
+        for p, g in zip(own, grads):
+            p.grad = None if g is None else g * factor
+        plain.step()
+        assert sum(g is not None for g in grads) >= 18
+        for p, old, new, ms in zip(own, before, after, moments):
+            assert torch.equal(p, new) and all(torch.equal(a, b) for a, b in zip(plain.moments(p), ms)), k
+            if bits == 32:
+                assert bool(((new - old).abs() <= (1.0 if k == 0 else 1.0014) * lr * (1 + 24 * 2.0 ** -24) + 2.0 ** -23 * old.abs()).all())
+        before = after
