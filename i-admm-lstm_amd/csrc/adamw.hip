@@ -10,7 +10,8 @@
 //
 // Measured (MI355X; a copy of 1 GiB runs at 5.3 TB/s on it), one tensor of 100 M elements: fp32 with 32 bits 522 us =
 // 5.4 TB/s, fp32 with 8 bits 299 us = 5.3, bf16 with 8 bits 194 us = 5.2 (where 47 vector instructions an element take
-// nearly as long as the memory); the 16 tensors of an h = 800 cell (2.6 M) 13.2 us, of an h = 200 cell 3.8 us.
+// nearly as long as the memory); mixed types at the same rate (32 bits: fp32 parameters with bf16 gradients 477 us, bf16
+// with fp32 442, bf16 with bf16 407 = 5.4 TB/s; 8 bits: fp32 with bf16 254, bf16 with fp32 226 = 5.3 to 5.5); the 16 tensors of an h = 800 cell (2.6 M) 13.2 us, of an h = 200 cell 3.8 us.
 //
 // 8-bit moments.  256 elements (a wave's 64 lanes with 4 each: its maximum needs no LDS) share two powers of
 // two.  m is a sign, 4 exponent and 3 mantissa bits under 2^em, v 5 and 3 bits without a sign under 2^ev:
@@ -595,7 +596,8 @@ __global__ void __launch_bounds__(1024) norm_end_kernel(const double* part, int 
 }
 
 // Workgroups take 2048 elements at a time up to this many in all, 8192 above: 168 000 of them 7.1 us against 7.7 (with the
-// last sum's launch; both since 1 us less), 2.6 M 8.2 against 8.0.
+// last sum's launch; both since 1 us less), 2.6 M 8.2 against 8.0.  Between these the two are within each other's spread
+// (GPU time in a graph: 100 000 4.3 against 4.9, 524 000 4.5 against 4.6, 1.2 M 4.8 against 4.9, 2.6 M 5.3 against 5.1).
 constexpr int64_t kNormSmall = int64_t{1} << 19;
 // Chunks of 1024 that one workgroup sums alone (16 waves, two rounds): 16 tensors of 2000 elements 5.8 us a call, 8.3 with
 // two launches; with four rounds the GPU takes longer than for the two.
@@ -651,7 +653,8 @@ __global__ void __launch_bounds__(1024) norm_few_kernel(const NormFew f) {
 }
 
 // Workgroups of 1024 elements up to this many in all, of 4096 above: 168 000 of them 7.9 us against 8.9 (with the
-// counting launch), 2.6 M 17.9 against 16.6.
+// counting launch), 2.6 M 17.9 against 16.6.  Between (GPU time in a graph, fp32 with 32 bits; bf16 with 8 in brackets):
+// 524 000 6.9 (6.6) against 7.8 (7.8), 1.2 M 9.1 (8.0) against 11.2 (11.1), 2.6 M 15.3 (10.3) against 14.7 (11.7).
 constexpr int64_t kAdamSmall = int64_t{1} << 19;
 template <bool EIGHT, int QUADS> static void launch_adam(const AdamLaunch& a, const AdamTensor* table, unsigned blocks,
                                                        hipStream_t st) {

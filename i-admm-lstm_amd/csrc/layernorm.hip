@@ -14,7 +14,9 @@
 // Measured (MI355X; a copy of 1 GiB runs at 5.3 TB/s on it): forward 256000 x 800 fp32 284 us = 5.8 TB/s, 8192 x 4096
 // bf16 24, 4000 x 800 fp32 6, one row 1.8; backward of the first three 436 (5.6 TB/s), 41 and 12 us with the slabs' sum.
 // 100 M elements, 100 to 16384 columns: forward 4.2 to 5.2 TB/s in 16 bits, 5.0 to 5.7 in 32; backward 3.9 to 5.1 and
-// 4.7 to 5.5, lowest where a row fills its threads badly (513, 1200 columns).
+// 4.7 to 5.5, lowest where a row fills its threads badly (513, 1200 columns).  100 M elements in longer rows: forward
+// 4.4 TB/s at 20000 to 30000 fp32 columns, 3.3 to 3.5 at 40000 to 50000 of 16 bits (8 vectors a thread), 2.3 at 100000 of
+// either, read again twice; backward 2.0 to 2.3 from 16385 on.
 #include <type_traits>
 
 #include "common.h"
@@ -261,7 +263,9 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) ln_fwd_kernel(LnFwd a) 
   if (lane == 0 && a.rstd) a.rstd[row] = r;
 }
 
-// Rows longer than the registers hold: a workgroup reads its row three times.
+// Rows longer than the registers hold (32768 fp32, 65536 16-bit elements): a workgroup reads its row three times, 4 e bytes
+// an element for 2 e, the second and third time from caches.  1000 x 100000: fp32 342 us, bf16 172 (2.3 TB/s of 2 e); 100
+// rows of a million fp32 836, as only 100 of 256 CUs have one.
 template <typename T> __global__ void __launch_bounds__(1024) ln_fwd_long_kernel(LnFwd a) {
   constexpr int V = Pack<T>::n, TPR = 1024;
   __shared__ float red[2][TPR / kWave];
@@ -556,8 +560,10 @@ constexpr int64_t kMaxCols = 1 << 24;  // (ln_slab_kernel's grid has 32 threads 
 constexpr int64_t kMaxHeld = 16384;  // elements of a row that a workgroup of the backward kernel holds
 
 // Forward: threads per row.  Fewer take their sums with less waiting, but each has more to load: up to 3 vectors each
-// in a wave, 4 beyond, 8 where there are no more threads (1500 columns of fp32: 64 threads 159 us for 400 MB, 128 147, 256 147 with half of them idle; 1200:
-// 150, 145, 149).  16 threads, whose sums stay among neighbours, with rows of 16 bits up to 5 vectors each (513 columns:
+// in a wave, 4 beyond, 8 where there are no more threads (1500 columns of fp32: 64 threads 159 us for 400 MB, 128 147, 256
+// 147 with half of them idle; 1200: 150, 145, 149; 8000: 512 threads with 4 vectors 150, 1024 with 3 160, at 7000 133 and
+// 130, 16000 of bf16 91 and 99; 16000 of fp32: 1024 threads with 4 145, with the 8 of longer rows 185; 24000 of fp32: 8
+// vectors 183, read three times 297, and 64 such rows of 30000 8.1 and 18.3).  16 threads, whose sums stay among neighbours, with rows of 16 bits up to 5 vectors each (513 columns:
 // 98 us for 200 MB, 64 threads 141; 800 columns: 86 and 82), of 32 bits up to 2 (400 columns: 163 and 139).
 static int row_threads_fwd(int64_t cols, int vec) {
   const int64_t n = (cols + vec - 1) / vec;
