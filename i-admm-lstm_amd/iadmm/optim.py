@@ -20,8 +20,9 @@ class AdamW(torch.optim.Optimizer):
     groups; ``norm`` holds the last one (0-dim device tensor).  ``.grad`` is not changed.
 
     ``capturable=True`` counts the steps on the device, so that a step captured into a graph counts its
-    replays; make one step before the capture (the state is allocated there).  A captured step keeps the
-    ``lr`` of its capture unless ``lr`` is a 1-element fp32 device tensor.
+    replays; make one step before the capture (the state is allocated there), and load a state before it (a loaded
+    state is other tensors than a captured step's).  A captured step keeps the ``lr`` of its capture unless ``lr`` is
+    a 1-element fp32 device tensor.
 
     Parameters without a gradient are left alone, as torch.optim does.  ``state_dict`` has torch.optim.AdamW's
     entries ("step", "exp_avg", "exp_avg_sq"; with 8 bits "exponents" too), and a state of torch.optim.AdamW, or of
@@ -41,7 +42,7 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"betas {betas}, eps {eps} or weight_decay {weight_decay} is out of range")
         self.state_bits, self.max_norm, self.seed, self.capturable = state_bits, max_norm, int(seed), bool(capturable)
         self.norm = None
-        self._counts = {}  # group index -> int64 device tensor of the steps made, and its elements by parameter (capturable)
+        self._counts = {}  # a group's first parameter -> int64 device tensor of the steps made, and its elements (capturable)
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
 
     def __getstate__(self):
@@ -51,7 +52,7 @@ class AdamW(torch.optim.Optimizer):
 
     def __setstate__(self, state):
         super().__setstate__(state)  # (load_state_dict comes here too, with the state and the groups)
-        self._counts = {}            # the next step gathers them from the parameters' "step"
+        self.__dict__.setdefault("_counts", {})  # (a copy's next step gathers them from the parameters' "step")
 
     def add_param_group(self, group):
         super().add_param_group(group)  # (params may be a generator: looked at where they are a list)
@@ -77,17 +78,20 @@ class AdamW(torch.optim.Optimizer):
                 s["exponents"] = torch.zeros(-(-p.numel() // ops.ADAM_BLOCK), 2, dtype=torch.int8, device=p.device)
         return s
 
-    def _count(self, gi, params):
+    def _count(self, params):
         """The group's steps as one device tensor, whose elements the parameters' "step" entries are."""
-        counts, own = self._counts.get(gi, (None, ()))
+        counts, own = self._counts.get(params[0], (None, ()))
         # (a copy of this optimizer, a changed group or a state put in from outside: entries that are not these elements)
         if len(own) != len(params) or any(self.state[p].get("step") is not c for p, c in zip(params, own)):
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("make one step before the capture: the steps' counts are not on the device yet")
             made = [int(self.state[p].get("step", 0)) for p in params]
-            counts = torch.tensor(made, dtype=torch.int64, device=params[0].device)
-            own = counts.unbind()
-            self._counts[gi] = counts, own
+            if len(own) == len(params) and counts.device == params[0].device:  # a captured step may hold its address
+                counts.copy_(torch.tensor(made))
+            else:
+                counts = torch.tensor(made, dtype=torch.int64, device=params[0].device)
+                own = counts.unbind()
+                self._counts[params[0]] = counts, own
             for p, c in zip(params, own):
                 self.state[p]["step"] = c
         return counts
@@ -114,7 +118,7 @@ class AdamW(torch.optim.Optimizer):
             # (with counts on the device every parameter has a state, also one that has had no gradient yet)
             states = [self._state(p) if self.capturable or x is not None else None for p, x in zip(params, gs)]
             if self.capturable:
-                step = self._count(gi, params)
+                step = self._count(params)
             else:
                 for s in states:
                     if s is not None and not isinstance(s["step"], int):
@@ -160,7 +164,6 @@ class AdamW(torch.optim.Optimizer):
                                      or s["exponents"].numel() != -(-p.numel() // ops.ADAM_BLOCK) * 2):
                 raise ValueError("not the codes and exponents of 8-bit moments (another optimizer may have cast them)")
         super().load_state_dict(state_dict)
-        self._counts = {}
         for g in self.param_groups:  # (Adam's mark: without a decay it loads, and the group is AdamW's from here on)
             g.pop("decoupled_weight_decay", None)
         for p, s in of:

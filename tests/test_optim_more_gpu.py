@@ -159,3 +159,41 @@ def test_clipping_inside_a_training_window(bits):
             if bits == 32:
                 assert bool(((new - old).abs() <= (1.0 if k == 0 else 1.0014) * lr * (1 + 24 * 2.0 ** -24) + 2.0 ** -23 * old.abs()).all())
         before = after
+
+
+def test_a_captured_step_counts_on_after_the_counts_were_gathered_again():
+    """Groups that changed places and a shallow copy's steps between the replays: the replays use and raise the parameters' own
+    counts, in the memory that they were captured with."""
+    from iadmm.optim import AdamW
+    a, b = params(), params()
+    groups = lambda ps: [dict(params=ps[:2]), dict(params=ps[2:], lr=3e-3)]  # noqa: E731
+    mine = AdamW(groups(a), lr=1e-2, betas=(0.5, 0.75), capturable=True)
+    host = AdamW(groups(b), lr=1e-2, betas=(0.5, 0.75))
+    set_grads(a[2:], 0)  # the groups' counts are apart
+    set_grads(b[2:], 0)
+    mine.step()
+    host.step()
+
+    def both(t, step):
+        set_grads(b, t)
+        for p, q in zip(a, b):
+            p.grad.copy_(q.grad)
+        step()
+        host.step()
+
+    set_grads(a, 1)
+    both(1, mine.step)
+    where = [mine.state[p]["step"].data_ptr() for p in a]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        mine.step()
+    shallow = copy.copy(mine)
+    for t, step in enumerate((graph.replay, shallow.step, mine.step, graph.replay, mine.step, graph.replay), 2):
+        if t == 6:
+            mine.param_groups.reverse()
+        both(t, step)
+        torch.cuda.synchronize()
+        for p, q in zip(a, b):  # (counts of the two kinds: corrections rounded apart, 2 u of an update)
+            assert bool(((p - q).abs() <= (t + 1) * 2.0 ** -24 * (4 * p.abs() + 24 * 2e-2)).all()), t
+    assert [int(mine.state[p]["step"]) for p in a] == [host.state[p]["step"] for p in b] == [7, 7, 8, 8, 8]
+    assert [mine.state[p]["step"].data_ptr() for p in a] == where
