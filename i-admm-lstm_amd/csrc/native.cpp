@@ -182,18 +182,19 @@ std::vector<Tensor> ln_backward(const Tensor& dy, const Tensor& x, const Tensor&
   return {dx, dw, db};
 }
 
-// A leaf's gradients are added up on the stream that its first living graph was made on.  Where that graph is older than a
-// capture, the engine would draw its stream into the capture, which ends the process: refused before it comes to that.
-void refuse_foreign_leaves(const c10::Device& d) {
+// A leaf's gradients are added up on the stream that its first living graph was made on, which a captured backward pass
+// draws into the capture.  Another stream joins it as a fork; the default stream cannot (the process ends): refused before it
+// comes to that.
+void refuse_default_stream_leaves(const c10::Device& d) {
   if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
   const auto node = torch::autograd::get_current_node();
   if (!node) return;
   for (const auto& edge : node->next_edges()) {
     const auto leaf = std::dynamic_pointer_cast<torch::autograd::AccumulateGrad>(edge.function);
     const auto stream = leaf ? leaf->stream() : std::nullopt;
-    TORCH_CHECK(!stream || (stream->device_index() == d.index() && stream->id() == c10::hip::getCurrentHIPStream(d.index()).id()),
-                "a captured backward pass of layer_norm needs its leaves for itself: a graph that was made from them before the "
-                "capture is still alive (delete its outputs, such as a loss, first)");
+    TORCH_CHECK(!stream || stream->id() != c10::hip::getDefaultHIPStream(d.index()).id(),
+                "a captured backward pass of layer_norm: a graph that was made on the default stream from the same leaves is "
+                "still alive (delete its outputs, such as a loss, before the capture)");
   }
 }
 
@@ -213,7 +214,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &w = saved[1];
     if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
-    refuse_foreign_leaves(x.device());
+    refuse_default_stream_leaves(x.device());
     const Tensor dy = plain_rows(grads[0]);  // (a sum's gradient is expanded)
     std::vector<Tensor> out;
     {

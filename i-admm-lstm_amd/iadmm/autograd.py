@@ -299,5 +299,5 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     :func:`iadmm.ops.layer_norm_bwd`.  x, and the gradient that reaches the output, may have any layout: copied where
     the rows are not contiguous, or where torch negates the view on reading.  Saves x and 8 bytes a row.  A C++
     autograd node (csrc/native.cpp), once differentiable; captured into a graph, its backward refuses leaves of which a
-    graph from before the capture is still alive."""
+    graph that was made on the default stream is still alive."""
     return _abi.native().layer_norm_grad(x, weight, bias, eps)

@@ -174,3 +174,32 @@ def test_tensors_without_memory_are_refused():
             call()
     torch.cuda.synchronize()
     assert torch.equal(x, keep) and int(counts) == 0
+
+
+def test_graphed_callable():
+    """torch.cuda.make_graphed_callables: forward and backward captured apart; a training loop's bits are the eager ones."""
+    from iadmm import autograd
+
+    class Norm(torch.nn.Module):
+        def __init__(self, w, b):
+            super().__init__()
+            self.w, self.b = (torch.nn.Parameter(p.detach().clone()) for p in (w, b))
+
+        def forward(self, x):
+            return autograd.layer_norm(x, self.w, self.b)
+
+    x, dy, w, b = inputs(333, 800)
+    plain, graphed = Norm(w, b), Norm(w, b)
+    call = torch.cuda.make_graphed_callables(graphed, (torch.zeros_like(x).requires_grad_(),))
+    for k in range(4):
+        x, dy, _, _ = inputs(333, 800, seed=k)
+        ends = []
+        for f, m in ((plain, plain), (call, graphed)):
+            for p in (x, m.w, m.b):
+                p.grad = None
+            y = f(x)
+            y.backward(dy)
+            ends.append([t.clone() for t in (y.detach(), x.grad, m.w.grad, m.b.grad)])
+            with torch.no_grad():
+                m.w -= 0.01 * m.w.grad
+        assert same(*ends), k
